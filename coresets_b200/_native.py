@@ -13,7 +13,7 @@ from typing import Optional
 
 from . import build as _build
 
-CS_ABI_VERSION = 9
+CS_ABI_VERSION = 10
 SELECT_SCRATCH_BYTES = 8192
 F_ELEMENT_ORDER = 1
 F_PDL = 2
@@ -40,6 +40,7 @@ EXPORTS = (
     "cs_reset_ctl", "cs_force_pick", "cs_commit_bound", "cs_fps_step", "cs_sim_begin",
     "cs_sim_final_check", "cs_xchg_window_words", "cs_xchg_wait", "cs_scan_argmax", "cs_fps_step_lanes", "cs_fps_step_noalloc",
     "cs_select_kth_largest", "cs_pool_argmax", "cs_cells_build", "cs_cells_select", "cs_fps_step_cells", "cs_force_pick_list", "cs_pool_pick",
+    "cs_rows8_write", "cs_rows8_read", "cs_rows8_take", "cs_rows8_products", "cs_rows8_coverage",
 )
 
 
@@ -90,6 +91,20 @@ class CsCells(ctypes.Structure):
         ("queue", ctypes.c_void_p),
         ("row_norm_max", ctypes.c_float),
         ("q_cap", ctypes.c_int32),
+    ]
+
+
+class CsRows8(ctypes.Structure):
+    """``cs_rows8`` of include/coresets_b200.h."""
+    _fields_ = [
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("norms", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("capacity", ctypes.c_int64),
+        ("count", ctypes.c_int64),
+        ("dim", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -176,6 +191,7 @@ class Native:
         L.cs_last_cuda_error.restype = ctypes.c_char_p
         L.cs_device_check.restype = ctypes.c_int
         sp = ctypes.POINTER(CsState)
+        rp = ctypes.POINTER(CsRows8)
         vp = ctypes.c_void_p
         for name, args in (
             ("cs_init_state", [sp, vp]),
@@ -195,6 +211,11 @@ class Native:
             ("cs_cells_build", [sp, ctypes.POINTER(CsCells), vp]),
             ("cs_cells_select", [sp, ctypes.POINTER(CsCells), vp]),
             ("cs_fps_step_cells", [sp, ctypes.POINTER(CsCells), vp]),
+            ("cs_rows8_write", [rp, vp, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, vp]),
+            ("cs_rows8_read", [rp, vp, ctypes.c_int64, vp, ctypes.c_int32, ctypes.c_int64, vp]),
+            ("cs_rows8_take", [rp, vp, ctypes.c_int64, rp, ctypes.c_int64, vp]),
+            ("cs_rows8_products", [rp, rp, vp, ctypes.c_int32, ctypes.c_int64, vp]),
+            ("cs_rows8_coverage", [rp, rp, vp, ctypes.c_int32, vp]),
         ):
             fn = getattr(L, name)
             fn.restype = ctypes.c_int
@@ -283,6 +304,21 @@ class Native:
 
     def fps_step_cells(self, s: CsState, c: CsCells, stream: int) -> None:
         self._check(self.lib.cs_fps_step_cells(ctypes.byref(s), ctypes.byref(c), stream), "cs_fps_step_cells")
+
+    def rows8_write(self, r: CsRows8, X: int, dtype: int, n: int, ld: int, start: int, stream: int) -> None:
+        self._check(self.lib.cs_rows8_write(ctypes.byref(r), X, dtype, n, ld, start, stream), "cs_rows8_write")
+
+    def rows8_read(self, r: CsRows8, rows: Optional[int], m: int, out: int, dtype: int, ld: int, stream: int) -> None:
+        self._check(self.lib.cs_rows8_read(ctypes.byref(r), rows, m, out, dtype, ld, stream), "cs_rows8_read")
+
+    def rows8_take(self, src: CsRows8, rows: int, m: int, dst: CsRows8, start: int, stream: int) -> None:
+        self._check(self.lib.cs_rows8_take(ctypes.byref(src), rows, m, ctypes.byref(dst), start, stream), "cs_rows8_take")
+
+    def rows8_products(self, a: CsRows8, b: CsRows8, out: int, dtype: int, ld: int, stream: int) -> None:
+        self._check(self.lib.cs_rows8_products(ctypes.byref(a), ctypes.byref(b), out, dtype, ld, stream), "cs_rows8_products")
+
+    def rows8_coverage(self, a: CsRows8, centres: CsRows8, h: int, keep: int, stream: int) -> None:
+        self._check(self.lib.cs_rows8_coverage(ctypes.byref(a), ctypes.byref(centres), h, keep, stream), "cs_rows8_coverage")
 
     def fps_step_lanes(self, lanes, n_lanes: int, mode: int, stream: int) -> None:
         self._check(self.lib.cs_fps_step_lanes(lanes, n_lanes, mode, stream), "cs_fps_step_lanes")

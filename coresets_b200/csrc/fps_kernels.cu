@@ -17,12 +17,17 @@
 //   small_kernels.cuh  state set-up kernels, stand-alone arg-max scan
 //   select.cuh         exact k-th largest, arg-max over a list of rows
 //   cells.cuh          cell index: rows grouped by centre, picks that read only the cells that can change
+//   rows8_store.cuh    rows in 8 bits: write, read back, copy
+//   rows8_mma.cuh      rows in 8 bits: products and distances on the tensor cores
+//   rows8_entry.cuh    rows in 8 bits: launchers and entry points
 //
 // Arithmetic is spelled with __fmul_rn/__fmaf_rn/__fadd_rn so that no compiler contraction or
 // reassociation can change a bit; the file is compiled with -ftz=true because the reference
 // builds with --use_fast_math (src/coresets/cuda/extension.py:63).
 #include "coresets_b200.h"
 
+#include <cuda.h>
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -39,6 +44,8 @@
 #include "small_kernels.cuh"
 #include "select.cuh"
 #include "cells.cuh"
+#include "rows8_store.cuh"
+#include "rows8_mma.cuh"
 
 namespace {
 
@@ -761,3 +768,5 @@ extern "C" int cs_fps_step_noalloc(const float* X, const float* norms, float* h,
                                             reinterpret_cast<u64*>(out_live_rows));
     return check_launch();
 }
+
+#include "rows8_entry.cuh"

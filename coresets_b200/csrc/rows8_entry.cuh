@@ -1,0 +1,242 @@
+// Rows in 8 bits: launchers and C entry points.
+// Part of the single translation unit fps_kernels.cu (included there, last).
+#ifndef CORESETS_B200_ROWS8_ENTRY_CUH
+#define CORESETS_B200_ROWS8_ENTRY_CUH
+
+namespace {
+
+int validate_rows8(const cs_rows8* r) {
+    if (!r || r->capacity < 0 || r->count < 0 || r->count > r->capacity || r->dim < 1) return CS_E_ARG;
+    if (r->capacity > 0 && (!r->codes || !r->scales || !r->norms)) return CS_E_ARG;
+    if (r->capacity >= (int64_t)1 << 31 || r->dim > CS_ROWS8_MAX_DIM) return CS_E_RANGE;
+    if (((uintptr_t)r->codes | (uintptr_t)r->scales | (uintptr_t)r->norms) & 15u) return CS_E_ALIGN;
+    return CS_OK;
+}
+
+int r8_grid(const int64_t groups, const DevInfo& d) {
+    const int64_t cap = (int64_t)d.sms * 8;                 // 2048 threads an SM
+    return (int)(groups < 1 ? 1 : (groups < cap ? groups : cap));
+}
+
+template <typename T, int G>
+int launch_rows8_write(const cs_rows8* r, const T* X, int64_t n, int64_t ld, int64_t start, cudaStream_t st, const DevInfo& d) {
+    const bool vec = ((uintptr_t)X & 15u) == 0 && (ld * sizeof(T)) % 16 == 0 && (r->dim & 7) == 0;
+    const int grid = r8_grid((n + kThreads / G - 1) / (kThreads / G), d);
+    if (vec) rows8_write_kernel<T, G, true><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    else rows8_write_kernel<T, G, false><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    return check_launch();
+}
+template <typename T>
+int launch_rows8_write(const cs_rows8* r, const void* X, int64_t n, int64_t ld, int64_t start, cudaStream_t st, const DevInfo& d) {
+    const T* x = static_cast<const T*>(X);
+    if (((uintptr_t)X % sizeof(T)) != 0) return CS_E_ALIGN;
+    // the lanes that 8 elements each of the row (its first block) take: padding codes up to the pitch are theirs too
+    if (r->dim <= 16) return launch_rows8_write<T, 2>(r, x, n, ld, start, st, d);
+    if (r->dim <= 32) return launch_rows8_write<T, 4>(r, x, n, ld, start, st, d);
+    if (r->dim <= 64) return launch_rows8_write<T, 8>(r, x, n, ld, start, st, d);
+    return launch_rows8_write<T, 16>(r, x, n, ld, start, st, d);
+}
+
+template <typename T, int G>
+int launch_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, T* out, int64_t ld, bool vec, cudaStream_t st, const DevInfo& d) {
+    const int grid = r8_grid((m + kThreads / G - 1) / (kThreads / G), d);
+    if (vec) rows8_read_kernel<T, G, true><<<grid, kThreads, 0, st>>>(*r, rows, m, out, ld);
+    else rows8_read_kernel<T, G, false><<<grid, kThreads, 0, st>>>(*r, rows, m, out, ld);
+    return check_launch();
+}
+template <typename T>
+int launch_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, void* out, int64_t ld, cudaStream_t st, const DevInfo& d) {
+    T* o = static_cast<T*>(out);
+    if (((uintptr_t)out % sizeof(T)) != 0) return CS_E_ALIGN;
+    constexpr int E = 16 / (int)sizeof(T);
+    const bool vec = ((uintptr_t)out & 15u) == 0 && (ld * sizeof(T)) % 16 == 0 && r->dim % E == 0;
+    const int chunks = vec ? r->dim / E : r->dim;
+    if (chunks <= 4) return launch_rows8_read<T, 4>(r, rows, m, o, ld, vec, st, d);
+    if (chunks <= 8) return launch_rows8_read<T, 8>(r, rows, m, o, ld, vec, st, d);
+    if (chunks <= 16) return launch_rows8_read<T, 16>(r, rows, m, o, ld, vec, st, d);
+    return launch_rows8_read<T, 32>(r, rows, m, o, ld, vec, st, d);
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// codes of the rows in use as tiles of `rows` x 128 bytes; what lies behind the last row or the pitch reads as 0
+int r8_map(CUtensorMap* map, const cs_rows8* r, const int rows) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return CS_E_DEVICE;
+    const cuuint64_t dims[2] = {(cuuint64_t)r8_pitch(r->dim), (cuuint64_t)r->count};
+    const cuuint64_t strides[1] = {(cuuint64_t)r8_pitch(r->dim)};
+    const cuuint32_t box[2] = {(cuuint32_t)kR8Block, (cuuint32_t)rows}, step[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r->codes, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? CS_OK
+               : CS_E_ARG;
+}
+
+template <int NT, int WHAT, typename T>
+int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
+    CUtensorMap lane_map, col_map;
+    int rc = r8_map(&lane_map, lanes, kR8Lanes);
+    if (rc) return rc;
+    rc = r8_map(&col_map, cols, NT);
+    if (rc) return rc;
+    static thread_local KernelTune tune;
+    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, R8Shape<NT>::kSmem, 192, nullptr);
+    if (rc) return rc;
+    job.col_tiles = (int)((job.n_col + NT - 1) / NT);
+    const int64_t lane_tiles = (job.n_lane + kR8Lanes - 1) / kR8Lanes;
+    if (WHAT == R8_PRODUCTS) {
+        job.col_split = 1;
+    } else {
+        // few lane tiles: split the centres until every SM has work
+        int64_t want = (d.sms + lane_tiles - 1) / lane_tiles;
+        want = want > job.col_tiles ? job.col_tiles : want;
+        job.col_split = (int)((job.col_tiles + want - 1) / want);
+    }
+    job.splits = (job.col_tiles + job.col_split - 1) / job.col_split;
+    job.items = lane_tiles * job.splits;
+    if (WHAT == R8_COVERAGE && job.splits > 1 && !job.keep) {
+        rows8_fill_kernel<<<r8_grid((job.n_lane + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(
+            static_cast<float*>(job.out), job.n_lane, __builtin_huge_valf());
+        rc = check_launch();
+        if (rc) return rc;
+    }
+    const int grid = (int)(job.items < d.sms ? job.items : d.sms);
+    rows8_mma_kernel<NT, WHAT, T><<<grid, 192, R8Shape<NT>::kSmem, st>>>(lane_map, col_map, job);
+    return check_launch();
+}
+// the narrowest tile that holds all columns, 128 where one does not
+template <int WHAT, typename T>
+int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
+    if (job.n_col <= 16) return launch_rows8_mma<16, WHAT, T>(lanes, cols, job, st, d);
+    if (job.n_col <= 32) return launch_rows8_mma<32, WHAT, T>(lanes, cols, job, st, d);
+    if (job.n_col <= 64) return launch_rows8_mma<64, WHAT, T>(lanes, cols, job, st, d);
+    return launch_rows8_mma<128, WHAT, T>(lanes, cols, job, st, d);
+}
+
+R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {
+    R8Job j = {};
+    j.lane_scales = static_cast<const unsigned char*>(lanes->scales);
+    j.col_scales = static_cast<const unsigned char*>(cols->scales);
+    j.lane_norms = lanes->norms;
+    j.col_norms = cols->norms;
+    j.n_lane = lanes->count;
+    j.n_col = cols->count;
+    j.D = lanes->dim;
+    j.words = r8_words(lanes->dim);
+    j.status = lanes->status;
+    return j;
+}
+
+}  // namespace
+
+extern "C" {
+
+int cs_rows8_write(const cs_rows8* r, const void* X, int32_t dtype, int64_t n, int64_t ld, int64_t start, cs_stream stream) {
+    int rc = validate_rows8(r);
+    if (rc) return rc;
+    if (n < 0 || start < 0 || start > r->capacity || n > r->capacity - start || (n > 0 && !X) || (n > 1 && ld < r->dim)) return CS_E_ARG;
+    if (dtype < CS_DTYPE_F32 || dtype > CS_DTYPE_BF16) return CS_E_ARG;
+    if (n == 0) return CS_OK;
+    DevInfo d = device_info();
+    if (!d.ok) return CS_E_DEVICE;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == CS_DTYPE_F32) return launch_rows8_write<float>(r, X, n, ld, start, st, d);
+    if (dtype == CS_DTYPE_F16) return launch_rows8_write<__half>(r, X, n, ld, start, st, d);
+    return launch_rows8_write<__nv_bfloat16>(r, X, n, ld, start, st, d);
+}
+
+int cs_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, void* out, int32_t dtype, int64_t ld, cs_stream stream) {
+    int rc = validate_rows8(r);
+    if (rc) return rc;
+    if (m < 0 || (m > 0 && !out) || (m > 1 && ld < r->dim) || (!rows && m > r->count)) return CS_E_ARG;
+    if (dtype < CS_DTYPE_F32 || dtype > CS_DTYPE_BF16) return CS_E_ARG;
+    if (m == 0) return CS_OK;
+    DevInfo d = device_info();
+    if (!d.ok) return CS_E_DEVICE;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == CS_DTYPE_F32) return launch_rows8_read<float>(r, rows, m, out, ld, st, d);
+    if (dtype == CS_DTYPE_F16) return launch_rows8_read<__half>(r, rows, m, out, ld, st, d);
+    return launch_rows8_read<__nv_bfloat16>(r, rows, m, out, ld, st, d);
+}
+
+int cs_rows8_take(const cs_rows8* src, const int64_t* rows, int64_t m, const cs_rows8* dst, int64_t start, cs_stream stream) {
+    int rc = validate_rows8(src);
+    if (rc) return rc;
+    rc = validate_rows8(dst);
+    if (rc) return rc;
+    if (src->dim != dst->dim || m < 0 || (m > 0 && !rows) || start < 0 || start > dst->capacity || m > dst->capacity - start) return CS_E_ARG;
+    if (m == 0) return CS_OK;
+    if (src->codes == dst->codes || src->scales == dst->scales) return CS_E_ARG;
+    DevInfo d = device_info();
+    if (!d.ok) return CS_E_DEVICE;
+    rows8_take_kernel<<<r8_grid((m + kWarps - 1) / kWarps, d), kThreads, 0, (cudaStream_t)stream>>>(*src, rows, m, *dst, start);
+    return check_launch();
+}
+
+int cs_rows8_products(const cs_rows8* a, const cs_rows8* b, void* out, int32_t dtype, int64_t ld, cs_stream stream) {
+    int rc = validate_rows8(a);
+    if (rc) return rc;
+    rc = validate_rows8(b);
+    if (rc) return rc;
+    if (a->dim != b->dim || dtype < CS_DTYPE_F32 || dtype > CS_DTYPE_BF16) return CS_E_ARG;
+    if (a->count == 0 || b->count == 0) return CS_OK;
+    if (!out || (a->count > 1 && ld < b->count)) return CS_E_ARG;
+    if ((uintptr_t)out % (dtype == CS_DTYPE_F32 ? 4u : 2u)) return CS_E_ALIGN;
+    DevInfo d = device_info();
+    if (!d.ok) return CS_E_DEVICE;
+    // lanes store consecutive elements of an output row when they are rows of b; with few rows of b most
+    // of the 128 lanes would be empty
+    const bool swap = b->count <= 64 && a->count > b->count;
+    const cs_rows8* lanes = swap ? a : b;
+    const cs_rows8* cols = swap ? b : a;
+    R8Job job = r8_job(lanes, cols);
+    job.out = out;
+    job.lane_stride = swap ? ld : 1;
+    job.col_stride = swap ? 1 : ld;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == CS_DTYPE_F32) return launch_rows8_mma<R8_PRODUCTS, float>(lanes, cols, job, st, d);
+    if (dtype == CS_DTYPE_F16) return launch_rows8_mma<R8_PRODUCTS, __half>(lanes, cols, job, st, d);
+    return launch_rows8_mma<R8_PRODUCTS, __nv_bfloat16>(lanes, cols, job, st, d);
+}
+
+int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int32_t keep, cs_stream stream) {
+    int rc = validate_rows8(a);
+    if (rc) return rc;
+    rc = validate_rows8(centres);
+    if (rc) return rc;
+    if (a->dim != centres->dim) return CS_E_ARG;
+    if (a->count == 0) return CS_OK;
+    if (!h) return CS_E_ARG;
+    if ((uintptr_t)h & 3u) return CS_E_ALIGN;
+    DevInfo d = device_info();
+    if (!d.ok) return CS_E_DEVICE;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (centres->count == 0) {
+        if (keep) return CS_OK;
+        rows8_fill_kernel<<<r8_grid((a->count + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(h, a->count, __builtin_huge_valf());
+        return check_launch();
+    }
+    R8Job job = r8_job(a, centres);
+    job.out = h;
+    job.keep = keep != 0;
+    return launch_rows8_mma<R8_COVERAGE, float>(a, centres, job, st, d);
+}
+
+}  // extern "C"
+
+#endif  // CORESETS_B200_ROWS8_ENTRY_CUH

@@ -1,0 +1,273 @@
+// Rows in 8 bits: products of the rows of two stores on the tensor cores, with the epilogues that use
+// them (the product itself; the distance of every row to the nearest centre).
+// Part of the single translation unit fps_kernels.cu (included there, in order).
+//
+//   P[i, j] = sum over blocks b of 128 of 2^(ea[i,b] + eb[j,b]) * sum over the block of a_i * b_j
+//
+// Powers of two are scales that tcgen05.mma kind::mxf8f6f4 applies by itself (one exponent byte per 32
+// elements of a row; the four quarters of a block of 128 name the same byte), so the whole sum over D
+// accumulates in TMEM in float32 and nothing has to be promoted between blocks.
+//
+// One block per SM: warp 0 copies (TMA, 128-byte swizzle; the exponents stand in the store in the
+// order that tcgen05.cp wants, 512 bytes per 128 rows and 4 blocks), warp 1 issues the MMAs, the other
+// warps read the accumulators back.  Rows of the "lane" operand are the 128 TMEM lanes of a tile, rows
+// of the "column" operand its NT columns.  Every wait is bounded; one that runs out sets the store's
+// status word and the whole block drains and leaves.
+#ifndef CORESETS_B200_ROWS8_MMA_CUH
+#define CORESETS_B200_ROWS8_MMA_CUH
+
+namespace {
+
+enum { R8_PRODUCTS = 0, R8_COVERAGE = 1 };
+constexpr int kR8Lanes = 128;                       // rows of the lane operand in a tile
+constexpr unsigned long long kR8WaitNs = 2000000000ull;
+
+struct R8Job {
+    const unsigned char* lane_scales;
+    const unsigned char* col_scales;
+    const float* lane_norms;                        // coverage only
+    const float* col_norms;
+    int64_t n_lane, n_col;                          // rows of the two operands
+    int D, words;
+    int col_tiles;                                  // tiles of NT columns
+    int col_split;                                  // column tiles of one work item
+    int splits;                                     // work items per lane tile
+    int64_t items;                                  // lane tiles * splits
+    void* out;                                      // products: P; coverage: h
+    int64_t lane_stride, col_stride;                // products, in elements
+    int keep;                                       // coverage: min with what h holds
+    int* status;
+};
+
+__device__ __forceinline__ uint64_t umma_desc(const uint32_t smem, const uint32_t stride_bytes, const uint64_t swizzle) {
+    // start >> 4, stride between groups of 8 rows >> 4, the constant 1 of this architecture, swizzle mode
+    return (uint64_t)((smem & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(stride_bytes >> 4) << 32) | (1ull << 46) | (swizzle << 61);
+}
+__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, const int x, const int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_copy_scales(const uint32_t tmem, const uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void tc_mma(const uint32_t acc, const uint64_t a, const uint64_t b, const uint32_t idesc,
+                                       const uint32_t sfa, const uint32_t sfb, const bool add) {
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %6, 0;\n"
+                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p; }"
+                 ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((unsigned)add) : "memory");
+}
+__device__ __forceinline__ void tc_load(const uint32_t tmem, unsigned (&u)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+                   "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]),
+                   "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]),
+                   "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+                 : "r"(tmem) : "memory");
+}
+__device__ __forceinline__ void tc_load(const uint32_t tmem, unsigned (&u)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+                   "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+                 : "r"(tmem) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// wait that also ends when another role has given up
+__device__ __forceinline__ bool r8_wait(uint64_t* b, const uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try(b, parity)) return true;
+    const unsigned long long t0 = global_ns();
+    for (;;) {
+#pragma unroll 1
+        for (int it = 0; it < 64; ++it)
+            if (mbar_try(b, parity)) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kR8WaitNs) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
+template <int NT> struct R8Shape {
+    static constexpr int kTileA = kR8Lanes * kR8Block, kTileB = NT * kR8Block;
+    static constexpr int kStage = kTileA + kTileB + 1024;              // two tiles, two scale words of 128 rows
+    static constexpr int kStages = NT >= 128 ? 6 : 8;
+    static constexpr int kSmem = kStages * kStage + 1024;              // slack to align the tiles to 1 KB
+};
+
+template <int NT, int WHAT, typename T>
+__global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant__ CUtensorMap lane_map,
+                                                           const __grid_constant__ CUtensorMap col_map, const R8Job job) {
+    using S = R8Shape<NT>;
+    constexpr int NC = NT < 32 ? NT : 32;                              // columns read back at a time
+    extern __shared__ unsigned char s_raw[];
+    __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort_word;
+    __shared__ __align__(16) float s_norm[4][NT < 32 ? 32 : NT];          // a copy per reading warp: no barrier between them
+    volatile int* s_abort = &s_abort_word;
+    unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kblocks = (job.D + kR8Block - 1) / kR8Block;
+    if (threadIdx.x == 0) {
+        s_abort_word = 0;
+        for (int i = 0; i < S::kStages; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 128); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    constexpr uint32_t kSf = 256;                                      // scale columns: 4 + 4 per stage behind the accumulators
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t n = 0;                                            // stages filled so far
+            bool ok = true;
+            for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
+                const int64_t lt = item / job.splits;
+                const int c0 = (int)(item % job.splits) * job.col_split;
+                const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
+                for (int ct = c0; ct < c1 && ok; ++ct)
+                    for (int kb = 0; kb < kblocks; ++kb, ++n) {
+                        const uint32_t st = n % S::kStages, round = n / S::kStages;
+                        if (round > 0 && !r8_wait(&s_empty[st], (round - 1) & 1u, s_abort)) { ok = false; break; }
+                        unsigned char* a = tiles + st * S::kStage;
+                        mbar_expect_tx(&s_full[st], S::kStage);
+                        tma_tile(a, &lane_map, kb * kR8Block, (int)(lt * kR8Lanes), &s_full[st]);
+                        tma_tile(a + S::kTileA, &col_map, kb * kR8Block, ct * NT, &s_full[st]);
+                        bulk_load(a + S::kTileA + S::kTileB, job.lane_scales + (lt * job.words + (kb >> 2)) * 512, 512, &s_full[st]);
+                        bulk_load(a + S::kTileA + S::kTileB + 512, job.col_scales + ((int64_t)(ct * NT >> 7) * job.words + (kb >> 2)) * 512,
+                                  512, &s_full[st]);
+                    }
+            }
+            // no copy may be in flight when the block leaves: the last fills of every stage (already
+            // complete unless a consumer gave up)
+            if (!ok)
+                for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
+                    for (int it = 0; it < (1 << 16) && !mbar_try(&s_full[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t n = 0, t = 0;
+            bool ok = true;
+            // e4m3 x e4m3, K-major, float32 accumulators, exponent-only scales, M = 128
+            constexpr uint32_t kIdesc = ((uint32_t)(NT >> 3) << 17) | (1u << 23) | ((uint32_t)(kR8Lanes >> 4) << 24);
+            for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
+                const int c0 = (int)(item % job.splits) * job.col_split;
+                const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
+                for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
+                    const uint32_t buf = t & 1u, round = t >> 1;
+                    if (round > 0 && !r8_wait(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t acc = tmem + buf * 128;
+                    for (int kb = 0; kb < kblocks; ++kb, ++n) {
+                        const uint32_t st = n % S::kStages;
+                        if (!r8_wait(&s_full[st], (n / S::kStages) & 1u, s_abort)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t a = smem_u32(tiles + st * S::kStage), b = a + S::kTileA, sf = b + S::kTileB;
+                        const uint32_t sfa = tmem + kSf + st * 8, sfb = sfa + 4;
+                        tc_copy_scales(sfa, umma_desc(sf, 128, 0));
+                        tc_copy_scales(sfb, umma_desc(sf + 512, 128, 0));
+                        const uint32_t id = kIdesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+                        const int left = job.D - kb * kR8Block, steps = left >= kR8Block ? 4 : (left + 31) >> 5;
+                        const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
+                        for (int k = 0; k < steps; ++k)
+                            tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, kb > 0 || k > 0);
+                        tc_commit(&s_empty[st]);
+                    }
+                    if (ok) tc_commit(&s_acc_full[buf]);
+                }
+            }
+            // the tensor core may still read the stages of a drained block: wait for what was issued
+            if (!ok)
+                for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
+                    for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
+        }
+    } else {
+        const int quad = warp & 3;
+        const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+        uint32_t t = 0;
+        bool ok = true;
+        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
+            const int64_t lt = item / job.splits;
+            const int c0 = (int)(item % job.splits) * job.col_split;
+            const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
+            const int64_t row = lt * kR8Lanes + quad * 32 + lane;
+            float best = __uint_as_float(0x7f800000u);
+            for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
+                const uint32_t buf = t & 1u;
+                if (WHAT == R8_COVERAGE) {
+                    // norms of the tile's centres; a column past the last centre can never be the nearest
+                    __syncwarp();
+                    for (int c = lane; c < NT; c += 32) {
+                        const int64_t col = (int64_t)ct * NT + c;
+                        s_norm[quad][c] = col < job.n_col ? __ldg(job.col_norms + col) : __uint_as_float(0x7f800000u);
+                    }
+                    __syncwarp();
+                }
+                if (!r8_wait(&s_acc_full[buf], (t >> 1) & 1u, s_abort)) ok = false;
+                ok = __all_sync(kFull, ok);
+                if (!ok) break;
+                tc_fence_after();
+                for (int c = 0; c < NT; c += NC) {
+                    unsigned v[NC];
+                    tc_load(lanes + buf * 128 + c, v);
+                    if (WHAT == R8_PRODUCTS) {
+                        const int64_t col = (int64_t)ct * NT + c;
+                        T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride + col * job.col_stride;
+                        if (row < job.n_lane) {
+#pragma unroll
+                            for (int j = 0; j < NC; ++j)
+                                if (col + j < job.n_col) {
+                                    T o;
+                                    r8_narrow(o, __uint_as_float(v[j]));
+                                    out[j * job.col_stride] = o;
+                                }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NC; ++j) best = fminf(best, __fmaf_rn(-2.0f, __uint_as_float(v[j]), s_norm[quad][c + j]));
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(&s_acc_empty[buf]);
+            }
+            if (WHAT == R8_COVERAGE && ok && row < job.n_lane) {
+                // |a - c|^2 = |a|^2 + (|c|^2 - 2 a.c); a NaN never lowers h, rounding never makes it negative
+                const float d = __fadd_rn(__ldg(job.lane_norms + row), best);
+                float* h = reinterpret_cast<float*>(job.out) + row;
+                const float up = d == d ? fmaxf(d, 0.0f) : __uint_as_float(0x7f800000u);
+                if (job.splits > 1) atomicMin(reinterpret_cast<int*>(h), __float_as_int(up));   // up >= 0: ordered like its bits, and below it every negative h
+                else *h = job.keep ? fminf(*h, up) : up;
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (threadIdx.x == 0 && s_abort_word && job.status) *job.status = ST_PIPE_TIMEOUT;
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+__global__ void rows8_fill_kernel(float* h, const int64_t n, const float v) {
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) h[i] = v;
+}
+
+}  // namespace
+
+#endif  // CORESETS_B200_ROWS8_MMA_CUH

@@ -2,19 +2,20 @@
 (src/coresets/cuda/fps.py:13-130)."""
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 from torch import Tensor
 
 from .. import engine as _engine
+from ..rows8 import RowStore, store_matrix
 
 # the CPU test-suite clears this to drive the host logic with a stand-in native library
 _REQUIRE_CUDA = True
 
 
 def fps(
-    X: Tensor,
+    X: Union[Tensor, RowStore],
     n_to_select: int,
     *,
     seed: Optional[Tensor] = None,
@@ -29,7 +30,15 @@ def fps(
 
     The whole loop runs on the device: per pick one bound kernel and one fused
     distance / min-update / arg-max kernel, replayed from a CUDA graph, no host read-back.
+
+    ``X`` may be a ``RowStore`` (an addition): its rows are read back once, exactly, and the picks are
+    those over the stored values with the store's own norms.
     """
+    norms = None
+    if isinstance(X, RowStore):
+        if not 1 <= n_to_select <= X.count:
+            raise ValueError(f"n_to_select={n_to_select} must be in [1, N={X.count}]")
+        norms, X = X.norms[: X.count], store_matrix(X)
     if _REQUIRE_CUDA and not X.is_cuda:
         raise ValueError(f"X must be on a CUDA device, got {X.device}")
     if X.dim() != 2:
@@ -54,7 +63,8 @@ def fps(
         seed_list = [0]
 
     X = X.contiguous()
-    norms = _engine.row_norms(X)                       # in X's own dtype, as fps.py:34 does
+    if norms is None:
+        norms = _engine.row_norms(X)                   # in X's own dtype, as fps.py:34 does
     X32, element_order = _engine.engine_matrix(X)
     eng = _engine.ShardEngine(X32, norms, n_to_select, element_order=element_order, cells=True)
     eng.init_state()

@@ -1,0 +1,297 @@
+"""Rows in 8 bits: a store of e4m3 rows with one power-of-two scale per 128 elements, and what works on it.
+
+    store = quantise_rows(X)                    # write (a whole matrix, or rows behind those it holds)
+    X = read_rows(store, rows, dtype=...)       # read rows back
+    P = row_products(a, b)                      # dot products of the rows of two stores
+    h = coverage(store, centres)                # squared distance of every row to its nearest centre
+    selected = fps_cuda(store, k)               # farthest points of the rows as stored
+
+No counterpart in the reference, whose rows have 16 bits at the least (src/coresets/cuda/kernels/warp.cu:167).
+An element takes one byte, and a row ``dim + 4 * ceil(dim / 512) + 4`` of them (``dim`` rounded up to 16): a quarter of
+float32.  The rounding to e4m3 is off by at most 2^-4 of an element, or 2^-10 of its block's scale; everything behind it works on
+the rows as stored, with float32 sums.
+
+Every call is enqueued on the current stream of the store's device, allocates nothing but its result (and a
+contiguous copy of an input whose columns are strided), synchronises with nothing and can be captured into
+a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+from torch import Tensor
+
+from . import _native
+from ._native import CsRows8
+
+BLOCK = 128
+MAX_DIM = 65536
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _dtype_code(dtype, what: str) -> int:
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+class _on:
+    """Make ``device`` current while a launch is enqueued; the stream is that device's current one."""
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.back = torch.cuda.current_device()
+        if self.back != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.back != self.index:
+            torch.cuda.set_device(self.back)
+
+
+class RowStore:
+    """Rows of ``dim`` elements in 8 bits, room for ``capacity`` of them, ``count`` (= ``len``) in use.
+
+    ``codes``  float8_e4m3fn [capacity, dim rounded up to 16];
+    ``scales`` uint8 [tiles of 128 rows, words, 32, 4, 4]: the exponent byte of block ``4 w + i`` of row
+    ``128 t + 32 j + r`` is ``scales[t, w, r, j, i]`` and its value 2^(byte - 127) -- the order in which the tensor
+    cores take scales (``exponents`` gives them row by row);
+    ``norms``  float32 [capacity], squared norms of the rows as stored."""
+
+    def __init__(self, capacity: int, dim: int, *, device=None):
+        capacity, dim = int(capacity), int(dim)
+        if capacity < 0 or capacity >= 2 ** 31:
+            raise ValueError(f"capacity={capacity} must be in [0, 2^31)")
+        if not 1 <= dim <= MAX_DIM:
+            raise ValueError(f"dim={dim} must be in [1, {MAX_DIM}]")
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise ValueError(f"a RowStore lives on a CUDA device, got {device}")
+        codes = torch.empty((capacity, (dim + 15) // 16 * 16), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        scales = torch.zeros((-(-capacity // 128), -(-dim // 512), 32, 4, 4), dtype=torch.uint8, device=device)
+        norms = torch.empty(capacity, dtype=torch.float32, device=device)
+        self._adopt(codes, scales, norms, dim, 0)
+
+    @classmethod
+    def from_tensors(cls, codes: Tensor, scales: Tensor, norms: Tensor, dim: int, *, count: Optional[int] = None) -> "RowStore":
+        """A store on arrays that are there already (loaded, or another store's); nothing is copied.  All
+        contiguous, shaped as the attributes of this class; ``count`` defaults to the capacity.  The codes
+        behind ``dim`` have to be 0."""
+        dim = int(dim)
+        if not 1 <= dim <= MAX_DIM:
+            raise ValueError(f"dim={dim} must be in [1, {MAX_DIM}]")
+        if codes.dim() != 2 or norms.dim() != 1:
+            raise ValueError(f"codes must be 2-D and norms 1-D, got shapes {tuple(codes.shape)} and {tuple(norms.shape)}")
+        capacity = codes.shape[0]
+        if capacity >= 2 ** 31:
+            raise ValueError(f"capacity={capacity} must be in [0, 2^31)")
+        want = {"codes": (codes, torch.float8_e4m3fn, (capacity, (dim + 15) // 16 * 16)),
+                "scales": (scales, torch.uint8, (-(-capacity // 128), -(-dim // 512), 32, 4, 4)),
+                "norms": (norms, torch.float32, (capacity,))}
+        for name, (t, dtype, shape) in want.items():
+            if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dtype} of shape {shape}, got {t.dtype} of shape {tuple(t.shape)}")
+            if not t.is_cuda or t.device != codes.device:
+                raise ValueError(f"{name} must be on one CUDA device with the others, got {t.device}")
+            if t.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned")
+        count = capacity if count is None else int(count)
+        if not 0 <= count <= capacity:
+            raise ValueError(f"count={count} must be in [0, capacity={capacity}]")
+        self = cls.__new__(cls)
+        self._adopt(codes, scales, norms, dim, count)
+        return self
+
+    def _adopt(self, codes, scales, norms, dim, count):
+        self.codes, self.scales, self.norms = codes, scales, norms
+        self.dim, self.capacity, self.device = dim, int(codes.shape[0]), codes.device
+        self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._c = CsRows8(codes.data_ptr(), scales.data_ptr(), norms.data_ptr(), self._status.data_ptr(),
+                          self.capacity, count, dim, 0)
+
+    @property
+    def count(self) -> int:
+        return self._c.count
+
+    def __len__(self) -> int:
+        return self._c.count
+
+    def __repr__(self) -> str:
+        return f"RowStore({self.count} of {self.capacity} rows x {self.dim}, {self.device})"
+
+    @property
+    def exponents(self) -> Tensor:
+        """uint8 [count, ceil(dim / 128)]: the exponent bytes row by row (a copy)."""
+        t, w = self.scales.shape[:2]
+        return self.scales.permute(0, 3, 2, 1, 4).reshape(t * 128, w * 4)[: self.count, : -(-self.dim // BLOCK)].contiguous()
+
+    def take(self, rows) -> "RowStore":
+        """A new store of the given rows, as they are (an index out of range: see ``read_rows``)."""
+        rows = _row_numbers(self, rows)
+        out = RowStore(rows.shape[0], self.dim, device=self.device)
+        with _on(self.device) as stream:
+            _native.get_native().rows8_take(self._c, rows.data_ptr(), rows.shape[0], out._c, 0, stream)
+        out._c.count = rows.shape[0]
+        return out
+
+    def check_status(self) -> None:
+        """Synchronise and raise if a bounded wait inside a product over this store ran out."""
+        status = int(self._status.item())
+        if status:
+            raise RuntimeError(f"a bounded wait of a product over {self!r} ran out (status {status}); its result is not valid")
+
+
+def _row_numbers(store: RowStore, rows) -> Tensor:
+    if not isinstance(rows, Tensor):
+        rows = torch.as_tensor(rows)
+        rows = rows.to(torch.int64) if rows.numel() == 0 else rows
+    if rows.dim() != 1 or rows.dtype.is_floating_point or rows.dtype.is_complex or rows.dtype == torch.bool:
+        raise ValueError(f"rows must be a 1-D tensor of whole numbers, got {rows.dtype} of shape {tuple(rows.shape)}")
+    if not rows.is_cuda:
+        if rows.numel() and not (0 <= int(rows.min()) and int(rows.max()) < store.count):
+            raise IndexError(f"rows must be in [0, {store.count}), got {int(rows.min())} .. {int(rows.max())}")
+    elif rows.device != store.device:
+        raise ValueError(f"rows are on {rows.device}, the store on {store.device}")
+    return rows.to(device=store.device, dtype=torch.int64).contiguous()
+
+
+def _check_store(store, name: str) -> RowStore:
+    if not isinstance(store, RowStore):
+        raise TypeError(f"{name} must be a RowStore (see quantise_rows), got {type(store).__name__}")
+    return store
+
+
+def quantise_rows(X: Tensor, *, store: Optional[RowStore] = None, start: Optional[int] = None) -> RowStore:
+    """Write the rows of ``X`` (float32, float16 or bfloat16, 2-D, on the device) into a store and return it.
+
+    Without ``store`` a new one of exactly these rows.  With it they go to rows ``start .. start + n``
+    (default: behind the rows it holds), over what stands there; the store has to have room for them and no
+    row before ``start`` may be unwritten.  Per block of 128 elements the scale is 2^e with the least e >= -117
+    for which every finite element fits e4m3 (448 at most); elements are rounded to nearest, ties to even.
+    NaN and infinities are stored as NaN.  No gradient flows through."""
+    if X.dim() != 2:
+        raise ValueError(f"X must be 2-D (N, D), got shape {tuple(X.shape)}")
+    if not X.is_cuda:
+        raise ValueError(f"X must be on a CUDA device, got {X.device}")
+    code = _dtype_code(X.dtype, "X.dtype")
+    if X.requires_grad and torch.is_grad_enabled():
+        raise ValueError("quantise_rows has no gradient: pass X.detach()")
+    n, dim = X.shape
+    if store is None:
+        if start:
+            raise ValueError("start needs a store")
+        store = RowStore(n, dim, device=X.device)
+    _check_store(store, "store")
+    if dim != store.dim:
+        raise ValueError(f"X has {dim} columns, the store {store.dim}")
+    if X.device != store.device:
+        raise ValueError(f"X is on {X.device}, the store on {store.device}")
+    start = store.count if start is None else int(start)
+    if not 0 <= start <= store.count:
+        raise ValueError(f"start={start} must be in [0, count={store.count}]: a store has no unwritten rows between others")
+    if start + n > store.capacity:
+        raise ValueError(f"rows {start} .. {start + n} do not fit the store's capacity {store.capacity}")
+    if n == 0:
+        return store
+    if (dim > 1 and X.stride(1) != 1) or (n > 1 and X.stride(0) < dim):
+        X = X.contiguous()
+    with _on(store.device) as stream:
+        _native.get_native().rows8_write(store._c, X.data_ptr(), code, n, X.stride(0) if n > 1 else dim, start, stream)
+    store._c.count = max(store._c.count, start + n)
+    return store
+
+
+def _result(out: Optional[Tensor], shape, dtype, device) -> Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"out must be {dtype} of shape {tuple(shape)} on {device}, got {out.dtype} of shape {tuple(out.shape)} on {out.device}")
+    if out.requires_grad:
+        raise ValueError("out must not require a gradient")
+    if (shape[1] > 1 and out.stride(1) != 1) or (shape[0] > 1 and out.stride(0) < shape[1]):
+        raise ValueError(f"out must have rows of consecutive elements that do not overlap, got strides {out.stride()}")
+    return out
+
+
+def read_rows(store: RowStore, rows=None, *, dtype: torch.dtype = torch.float32, out: Optional[Tensor] = None) -> Tensor:
+    """Rows of the store as ``dtype`` (exact in float32 and bfloat16, rounded once in float16).
+
+    ``rows``: whole numbers in any order, repeats allowed; default all rows.  Numbers that the host holds are
+    checked (``IndexError``); numbers on the device are not, and one outside ``[0, count)`` gives a row of NaN."""
+    _check_store(store, "store")
+    code = _dtype_code(dtype, "dtype")
+    if rows is not None:
+        rows = _row_numbers(store, rows)
+    m = store.count if rows is None else rows.shape[0]
+    out = _result(out, (m, store.dim), dtype, store.device)
+    if m:
+        with _on(store.device) as stream:
+            _native.get_native().rows8_read(store._c, None if rows is None else rows.data_ptr(), m, out.data_ptr(), code,
+                                            out.stride(0) if m > 1 else store.dim, stream)
+    return out
+
+
+def _check_pair(a: RowStore, b: RowStore, names) -> None:
+    _check_store(a, names[0])
+    _check_store(b, names[1])
+    if a.dim != b.dim:
+        raise ValueError(f"{names[0]} has rows of {a.dim} elements, {names[1]} of {b.dim}")
+    if a.device != b.device:
+        raise ValueError(f"{names[0]} is on {a.device}, {names[1]} on {b.device}")
+
+
+def row_products(a: RowStore, b: RowStore, *, dtype: torch.dtype = torch.float32, out: Optional[Tensor] = None) -> Tensor:
+    """``[len(a), len(b)]``: the dot product of every row of ``a`` with every row of ``b``, summed in float32 and
+    rounded once to ``dtype``."""
+    _check_pair(a, b, ("a", "b"))
+    code = _dtype_code(dtype, "dtype")
+    n, k = a.count, b.count
+    out = _result(out, (n, k), dtype, a.device)
+    if n and k:
+        with _on(a.device) as stream:
+            _native.get_native().rows8_products(a._c, b._c, out.data_ptr(), code, out.stride(0) if n > 1 else k, stream)
+    return out
+
+
+def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
+    """float32 ``[len(store)]``: the squared distance of every row to the nearest of ``centres`` (a store, or
+    numbers of rows of this one); its maximum is the squared Hausdorff radius of the selection.
+
+    With ``h`` the minimum is taken with what ``h`` holds, in place: a selection can be passed part by part,
+    and rows that carry -1 (selected) keep it.  A distance is never negative, one that is NaN never lowers ``h``, and
+    without centres ``h`` is +inf."""
+    _check_store(store, "store")
+    if not isinstance(centres, RowStore):
+        centres = store.take(centres)
+    _check_pair(store, centres, ("store", "centres"))
+    n = store.count
+    keep = h is not None
+    if keep:
+        if h.dtype != torch.float32 or tuple(h.shape) != (n,) or h.device != store.device or not h.is_contiguous():
+            raise ValueError(f"h must be contiguous float32 of shape ({n},) on {store.device}, got {h.dtype} of shape {tuple(h.shape)} on {h.device}")
+        if h.requires_grad:
+            raise ValueError("h must not require a gradient")
+    else:
+        h = torch.empty(n, dtype=torch.float32, device=store.device)
+    if n:
+        with _on(store.device) as stream:
+            _native.get_native().rows8_coverage(store._c, centres._c, h.data_ptr(), int(keep), stream)
+    return h
+
+
+def store_matrix(store: RowStore) -> Tensor:
+    """The store's rows as a matrix that the selection kernels read, holding exactly the stored values: float16 where
+    every exponent lets it (2 bytes an element), float32 otherwise.  Reads two numbers back to the host."""
+    e = store.exponents
+    if e.numel():
+        low, high = (int(v) - 127 for v in torch.stack(torch.aminmax(e)).tolist())
+        # code * 2^e is a multiple of 2^(e - 9) and at most 448 * 2^e; float16 has multiples of 2^-24 up to 65504
+        if low >= -15 and high <= 7:
+            return read_rows(store, dtype=torch.float16)
+    return read_rows(store, dtype=torch.float32)

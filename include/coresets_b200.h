@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define CS_ABI_VERSION 9
+#define CS_ABI_VERSION 10
 
 #if defined(__GNUC__)
 #define CS_API __attribute__((visibility("default")))
@@ -389,6 +389,60 @@ CS_API int cs_fps_step_noalloc(const float* X, const float* norms, float* h, int
                                int64_t N_local, int32_t D, int64_t shard_offset, const float* centre,
                                float norm_new, const float* dSL_quarter, int32_t sel_pos, uint32_t mode,
                                uint64_t* out_key, uint64_t* out_live_rows, cs_stream stream);
+
+/*
+ * Rows in 8 bits.  A store keeps rows of `dim` elements as e4m3 codes with one power-of-two scale per
+ * 128 elements, and the squared norm of each row as stored.  No counterpart in the reference, which
+ * reads float16 at the least (kernels/warp.cu:167).
+ *
+ *   codes   [capacity, pitch] bytes, pitch = dim rounded up to 16; the codes behind dim are 0
+ *   scales  [tiles of 128 rows, words, 32, 4, 4] bytes, words = ceil(dim / 512): the exponent byte of block
+ *           4 w + i of row 128 t + 32 j + r stands at [t, w, r, j, i]; value 2^(byte - 127), 255 = NaN
+ *   norms   [capacity] floats
+ *
+ * Every row of the last tile has its scale bytes, written or not (zero them once).  All pointers
+ * 16-byte aligned.  Rows < 2^31, dim <= CS_ROWS8_MAX_DIM.
+ */
+#define CS_ROWS8_MAX_DIM 65536
+#define CS_DTYPE_F32 0
+#define CS_DTYPE_F16 1
+#define CS_DTYPE_BF16 2
+typedef struct cs_rows8 {
+    void* codes;
+    void* scales;
+    float* norms;
+    int32_t* status;     /* device word, set to 4 when a bounded wait of a product ran out; may be NULL */
+    int64_t capacity;    /* rows that the arrays hold                                                */
+    int64_t count;       /* rows in use: what reads and products take                                 */
+    int32_t dim;
+    int32_t reserved;
+} cs_rows8;
+
+/* Quantise n rows of X (dtype CS_DTYPE_*, row stride ld elements) into rows start .. start + n of the
+ * store (start + n <= capacity; `count` is not looked at).  e = the least integer with amax <= 448 * 2^e
+ * over the block's finite elements, at least -117; code = e4m3(x * 2^-e) to nearest even; NaN and
+ * infinities become the NaN code.  Other rows are left as they were. */
+CS_API int cs_rows8_write(const cs_rows8* r, const void* X, int32_t dtype, int64_t n, int64_t ld, int64_t start,
+                          cs_stream stream);
+
+/* out[i] = row rows[i] of the store (rows NULL: row i), m rows of row stride ld elements, rounded once to
+ * the output type.  A row number outside [0, count) gives a row of NaN. */
+CS_API int cs_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, void* out, int32_t dtype, int64_t ld,
+                         cs_stream stream);
+
+/* Copy rows rows[0..m) of src, as they are, to rows start .. start + m of dst (same dim, other memory).
+ * A row number outside [0, src->count) gives a row of NaN. */
+CS_API int cs_rows8_take(const cs_rows8* src, const int64_t* rows, int64_t m, const cs_rows8* dst, int64_t start,
+                         cs_stream stream);
+
+/* out[i * ld + j] = dot(row i of a, row j of b), float32 accumulation, rounded once to the output type. */
+CS_API int cs_rows8_products(const cs_rows8* a, const cs_rows8* b, void* out, int32_t dtype, int64_t ld,
+                             cs_stream stream);
+
+/* h[i] = min over the centres j of max(0, norms_a[i] + norms_c[j] - 2 dot(i, j)), i in [0, a->count); with
+ * keep != 0 also over what h[i] holds (rows that carry -1 keep it).  A distance that is NaN never lowers
+ * h; without centres h is +inf (keep == 0). */
+CS_API int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int32_t keep, cs_stream stream);
 
 #ifdef __cplusplus
 }
