@@ -19,6 +19,7 @@
 //   cells.cuh          cell index: rows grouped by centre, picks that read only the cells that can change
 //   rows8_store.cuh    rows in 8 bits: write, read back, copy
 //   rows8_mma.cuh      rows in 8 bits: products and distances on the tensor cores
+//   rows8_pair.cuh     the same for many columns, on pairs of SMs
 //   rows8_entry.cuh    rows in 8 bits: launchers and entry points
 //
 // Arithmetic is spelled with __fmul_rn/__fmaf_rn/__fadd_rn so that no compiler contraction or
@@ -46,6 +47,7 @@
 #include "cells.cuh"
 #include "rows8_store.cuh"
 #include "rows8_mma.cuh"
+#include "rows8_pair.cuh"
 
 namespace {
 

@@ -87,6 +87,55 @@ int r8_map(CUtensorMap* map, const cs_rows8* r, const int rows) {
                : CS_E_ARG;
 }
 
+// the scale words of 128 rows as rows of 512 bytes, `chunks` consecutive tiles of 128 rows at once
+int r8_scale_map(CUtensorMap* map, const cs_rows8* r, const int chunks) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return CS_E_DEVICE;
+    const cuuint64_t words = (cuuint64_t)r8_words(r->dim);
+    const cuuint64_t dims[3] = {128, words, (cuuint64_t)((r->count + 127) / 128)};
+    const cuuint64_t strides[2] = {512, words * 512};
+    const cuuint32_t box[3] = {128, 1, (cuuint32_t)chunks}, step[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, r->scales, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? CS_OK
+               : CS_E_ARG;
+}
+
+template <int WHAT, typename T>
+int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
+    CUtensorMap lane_map, col_map, lane_sf, col_sf;
+    int rc = r8_map(&lane_map, lanes, kR8Lanes);
+    if (rc) return rc;
+    rc = r8_map(&col_map, cols, kPairCols / 2);
+    if (rc) return rc;
+    rc = r8_scale_map(&lane_sf, lanes, 1);
+    if (rc) return rc;
+    rc = r8_scale_map(&col_sf, cols, 2);
+    if (rc) return rc;
+    static thread_local KernelTune tune;
+    rc = tune_kernel(rows8_pair_kernel<WHAT, T>, tune, d.dev, kPairSmem, kPairWarps * 32, nullptr);
+    if (rc) return rc;
+    const int64_t pairs = d.sms / 2, lane_tiles = (job.n_lane + kPairLanes - 1) / kPairLanes;
+    job.col_tiles = (int)((job.n_col + kPairCols - 1) / kPairCols);
+    job.col_split = 1;
+    if (WHAT == R8_COVERAGE) {
+        int64_t want = (pairs + lane_tiles - 1) / lane_tiles;
+        want = want > job.col_tiles ? job.col_tiles : want;
+        job.col_split = (int)((job.col_tiles + want - 1) / want);
+    }
+    job.splits = (job.col_tiles + job.col_split - 1) / job.col_split;
+    job.items = lane_tiles * job.splits;
+    if (WHAT == R8_COVERAGE && !job.keep) {
+        rows8_fill_kernel<<<r8_grid((job.n_lane + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(
+            static_cast<float*>(job.out), job.n_lane, __builtin_huge_valf());
+        rc = check_launch();
+        if (rc) return rc;
+    }
+    const int grid = 2 * (int)(job.items < pairs ? job.items : pairs);
+    rows8_pair_kernel<WHAT, T><<<grid, kPairWarps * 32, kPairSmem, st>>>(lane_map, col_map, lane_sf, col_sf, job);
+    return check_launch();
+}
+
 template <int NT, int WHAT, typename T>
 int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
     CUtensorMap lane_map, col_map;
@@ -119,13 +168,14 @@ int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cu
     rows8_mma_kernel<NT, WHAT, T><<<grid, 192, R8Shape<NT>::kSmem, st>>>(lane_map, col_map, job);
     return check_launch();
 }
-// the narrowest tile that holds all columns, 128 where one does not
+// the narrowest tile that holds all columns; pairs of SMs where 64 do not (coverage of 1M x 128 by 8192 centres:
+// 1.28 ms, with tiles of 128 x 128 on single SMs 3.11 ms)
 template <int WHAT, typename T>
 int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
     if (job.n_col <= 16) return launch_rows8_mma<16, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 32) return launch_rows8_mma<32, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 64) return launch_rows8_mma<64, WHAT, T>(lanes, cols, job, st, d);
-    return launch_rows8_mma<128, WHAT, T>(lanes, cols, job, st, d);
+    return launch_rows8_pair<WHAT, T>(lanes, cols, job, st, d);
 }
 
 R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {

@@ -1,5 +1,6 @@
 // Rows in 8 bits: products of the rows of two stores on the tensor cores, with the epilogues that use
-// them (the product itself; the distance of every row to the nearest centre).
+// them (the product itself; the distance of every row to the nearest centre).  This file: few columns
+// (at most 64), which all stand in one tile; rows8_pair.cuh: many.
 // Part of the single translation unit fps_kernels.cu (included there, in order).
 //
 //   P[i, j] = sum over blocks b of 128 of 2^(ea[i,b] + eb[j,b]) * sum over the block of a_i * b_j
@@ -79,26 +80,43 @@ __device__ __forceinline__ void tc_load(const uint32_t tmem, unsigned (&u)[16]) 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// wait that also ends when another role has given up
+// One lane of a converged warp.  The copy and MMA instructions take their descriptors from uniform
+// registers: under a branch that the compiler cannot see to be one lane's each of them costs ~230 clocks
+// (products 8192^3: 968 us that way), so the warps' loops run converged and only the issue is elected.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p != 0;
+}
+
+// Wait that also ends when another role has given up.  The clock is looked at only after many tries (each
+// of which the hardware may itself hold for a while): reading it costs more than most waits last.
 __device__ __forceinline__ bool r8_wait(uint64_t* b, const uint32_t parity, volatile int* abort_flag) {
     if (mbar_try(b, parity)) return true;
-    const unsigned long long t0 = global_ns();
+    unsigned long long t0 = 0;
     for (;;) {
 #pragma unroll 1
-        for (int it = 0; it < 64; ++it)
+        for (int it = 0; it < 1024; ++it)
             if (mbar_try(b, parity)) return true;
         if (*abort_flag) return false;
-        if (global_ns() - t0 > kR8WaitNs) {
+        const unsigned long long now = global_ns();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > kR8WaitNs) {
             *abort_flag = 1;
             return false;
         }
     }
 }
 
+// the same by a whole converged warp
+__device__ __forceinline__ bool r8_wait_warp(uint64_t* b, const uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(kFull, r8_wait(b, parity, abort_flag));
+}
+
 template <int NT> struct R8Shape {
     static constexpr int kTileA = kR8Lanes * kR8Block, kTileB = NT * kR8Block;
     static constexpr int kStage = kTileA + kTileB + 1024;              // two tiles, two scale words of 128 rows
-    static constexpr int kStages = NT >= 128 ? 6 : 8;
+    static constexpr int kStages = 8;
     static constexpr int kSmem = kStages * kStage + 1024;              // slack to align the tiles to 1 KB
 };
 
@@ -115,7 +133,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
     volatile int* s_abort = &s_abort_word;
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;    // warp: known to be uniform
     const int kblocks = (job.D + kR8Block - 1) / kR8Block;
     if (threadIdx.x == 0) {
         s_abort_word = 0;
@@ -130,22 +148,22 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(kFull, s_tmem, 0);
     constexpr uint32_t kSf = 256;                                      // scale columns: 4 + 4 per stage behind the accumulators
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t n = 0;                                            // stages filled so far
-            bool ok = true;
-            for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
-                const int64_t lt = item / job.splits;
-                const int c0 = (int)(item % job.splits) * job.col_split;
-                const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
-                for (int ct = c0; ct < c1 && ok; ++ct)
-                    for (int kb = 0; kb < kblocks; ++kb, ++n) {
-                        const uint32_t st = n % S::kStages, round = n / S::kStages;
-                        if (round > 0 && !r8_wait(&s_empty[st], (round - 1) & 1u, s_abort)) { ok = false; break; }
-                        unsigned char* a = tiles + st * S::kStage;
+        uint32_t n = 0;                                                // stages filled so far
+        bool ok = true;
+        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
+            const int64_t lt = item / job.splits;
+            const int c0 = (int)(item % job.splits) * job.col_split;
+            const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
+            for (int ct = c0; ct < c1 && ok; ++ct)
+                for (int kb = 0; kb < kblocks; ++kb, ++n) {
+                    const uint32_t st = n % S::kStages, round = n / S::kStages;
+                    if (round > 0 && !r8_wait_warp(&s_empty[st], (round - 1) & 1u, s_abort)) { ok = false; break; }
+                    unsigned char* a = tiles + st * S::kStage;
+                    if (elect_one()) {
                         mbar_expect_tx(&s_full[st], S::kStage);
                         tma_tile(a, &lane_map, kb * kR8Block, (int)(lt * kR8Lanes), &s_full[st]);
                         tma_tile(a + S::kTileA, &col_map, kb * kR8Block, ct * NT, &s_full[st]);
@@ -153,31 +171,31 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
                         bulk_load(a + S::kTileA + S::kTileB + 512, job.col_scales + ((int64_t)(ct * NT >> 7) * job.words + (kb >> 2)) * 512,
                                   512, &s_full[st]);
                     }
-            }
-            // no copy may be in flight when the block leaves: the last fills of every stage (already
-            // complete unless a consumer gave up)
-            if (!ok)
-                for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
-                    for (int it = 0; it < (1 << 16) && !mbar_try(&s_full[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
+                    __syncwarp();
+                }
         }
+        // no copy may be in flight when the block leaves: the last fills of every stage (already
+        // complete unless a consumer gave up)
+        if (!ok)
+            for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
+                for (int it = 0; it < (1 << 16) && !mbar_try(&s_full[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t n = 0, t = 0;
-            bool ok = true;
-            // e4m3 x e4m3, K-major, float32 accumulators, exponent-only scales, M = 128
-            constexpr uint32_t kIdesc = ((uint32_t)(NT >> 3) << 17) | (1u << 23) | ((uint32_t)(kR8Lanes >> 4) << 24);
-            for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
-                const int c0 = (int)(item % job.splits) * job.col_split;
-                const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
-                for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
-                    const uint32_t buf = t & 1u, round = t >> 1;
-                    if (round > 0 && !r8_wait(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
+        uint32_t n = 0, t = 0;
+        bool ok = true;
+        // e4m3 x e4m3, K-major, float32 accumulators, exponent-only scales, M = 128
+        constexpr uint32_t kIdesc = ((uint32_t)(NT >> 3) << 17) | (1u << 23) | ((uint32_t)(kR8Lanes >> 4) << 24);
+        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
+            const int c0 = (int)(item % job.splits) * job.col_split;
+            const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
+            for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
+                const uint32_t buf = t & 1u, round = t >> 1;
+                if (round > 0 && !r8_wait_warp(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
+                const uint32_t acc = tmem + buf * 128;
+                for (int kb = 0; kb < kblocks; ++kb, ++n) {
+                    const uint32_t st = n % S::kStages;
+                    if (!r8_wait_warp(&s_full[st], (n / S::kStages) & 1u, s_abort)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t acc = tmem + buf * 128;
-                    for (int kb = 0; kb < kblocks; ++kb, ++n) {
-                        const uint32_t st = n % S::kStages;
-                        if (!r8_wait(&s_full[st], (n / S::kStages) & 1u, s_abort)) { ok = false; break; }
-                        tc_fence_after();
+                    if (elect_one()) {
                         const uint32_t a = smem_u32(tiles + st * S::kStage), b = a + S::kTileA, sf = b + S::kTileB;
                         const uint32_t sfa = tmem + kSf + st * 8, sfb = sfa + 4;
                         tc_copy_scales(sfa, umma_desc(sf, 128, 0));
@@ -188,15 +206,16 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
                         for (int k = 0; k < steps; ++k)
                             tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, kb > 0 || k > 0);
                         tc_commit(&s_empty[st]);
+                        if (kb == kblocks - 1) tc_commit(&s_acc_full[buf]);
                     }
-                    if (ok) tc_commit(&s_acc_full[buf]);
+                    __syncwarp();
                 }
             }
-            // the tensor core may still read the stages of a drained block: wait for what was issued
-            if (!ok)
-                for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
-                    for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
         }
+        // the tensor core may still read the stages of a drained block: wait for what was issued
+        if (!ok)
+            for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
+                for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
     } else {
         const int quad = warp & 3;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
@@ -219,8 +238,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
                     }
                     __syncwarp();
                 }
-                if (!r8_wait(&s_acc_full[buf], (t >> 1) & 1u, s_abort)) ok = false;
-                ok = __all_sync(kFull, ok);
+                ok = r8_wait_warp(&s_acc_full[buf], (t >> 1) & 1u, s_abort);
                 if (!ok) break;
                 tc_fence_after();
                 for (int c = 0; c < NT; c += NC) {
