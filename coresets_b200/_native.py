@@ -40,7 +40,7 @@ EXPORTS = (
     "cs_reset_ctl", "cs_force_pick", "cs_commit_bound", "cs_fps_step", "cs_sim_begin",
     "cs_sim_final_check", "cs_xchg_window_words", "cs_xchg_wait", "cs_scan_argmax", "cs_fps_step_lanes", "cs_fps_step_noalloc",
     "cs_select_kth_largest", "cs_pool_argmax", "cs_cells_build", "cs_cells_select", "cs_fps_step_cells", "cs_force_pick_list", "cs_pool_pick",
-    "cs_rows8_write", "cs_rows8_read", "cs_rows8_take", "cs_rows8_products", "cs_rows8_coverage",
+    "cs_rows8_write", "cs_rows8_read", "cs_rows8_take", "cs_rows8_products", "cs_rows8_coverage", "cs_rows8_coverage_bytes",
 )
 
 
@@ -215,13 +215,15 @@ class Native:
             ("cs_rows8_read", [rp, vp, ctypes.c_int64, vp, ctypes.c_int32, ctypes.c_int64, vp]),
             ("cs_rows8_take", [rp, vp, ctypes.c_int64, rp, ctypes.c_int64, vp]),
             ("cs_rows8_products", [rp, rp, vp, ctypes.c_int32, ctypes.c_int64, vp]),
-            ("cs_rows8_coverage", [rp, rp, vp, ctypes.c_int32, vp]),
+            ("cs_rows8_coverage", [rp, rp, vp, ctypes.c_int32, vp, vp]),
         ):
             fn = getattr(L, name)
             fn.restype = ctypes.c_int
             fn.argtypes = args
         L.cs_xchg_window_words.restype = ctypes.c_int64
         L.cs_xchg_window_words.argtypes = [ctypes.c_int32, ctypes.c_int32]
+        L.cs_rows8_coverage_bytes.restype = ctypes.c_int64
+        L.cs_rows8_coverage_bytes.argtypes = [ctypes.c_int64]
         L.cs_fps_step_noalloc.restype = ctypes.c_int
         L.cs_fps_step_noalloc.argtypes = [vp, vp, vp, vp, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, vp,
                                           ctypes.c_float, vp, ctypes.c_int32, ctypes.c_uint32, vp, vp, vp]
@@ -317,8 +319,9 @@ class Native:
     def rows8_products(self, a: CsRows8, b: CsRows8, out: int, dtype: int, ld: int, stream: int) -> None:
         self._check(self.lib.cs_rows8_products(ctypes.byref(a), ctypes.byref(b), out, dtype, ld, stream), "cs_rows8_products")
 
-    def rows8_coverage(self, a: CsRows8, centres: CsRows8, h: int, keep: int, stream: int) -> None:
-        self._check(self.lib.cs_rows8_coverage(ctypes.byref(a), ctypes.byref(centres), h, keep, stream), "cs_rows8_coverage")
+    def rows8_coverage(self, a: CsRows8, centres: CsRows8, h: int, keep: int, work: Optional[int],
+                       stream: int) -> None:
+        self._check(self.lib.cs_rows8_coverage(ctypes.byref(a), ctypes.byref(centres), h, keep, work, stream), "cs_rows8_coverage")
 
     def fps_step_lanes(self, lanes, n_lanes: int, mode: int, stream: int) -> None:
         self._check(self.lib.cs_fps_step_lanes(lanes, n_lanes, mode, stream), "cs_fps_step_lanes")

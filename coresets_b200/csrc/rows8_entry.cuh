@@ -74,74 +74,81 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
-// codes of the rows in use as tiles of `rows` x 128 bytes; what lies behind the last row or the pitch reads as 0
-int r8_map(CUtensorMap* map, const cs_rows8* r, const int rows) {
+// rows of `dim` bytes as tiles of `rows` x `width`; what lies behind the last row or the pitch reads as 0
+int r8_map(CUtensorMap* map, void* base, const int dim, const int64_t count, const int width, const int rows, const bool swizzle) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return CS_E_DEVICE;
-    const cuuint64_t dims[2] = {(cuuint64_t)r8_pitch(r->dim), (cuuint64_t)r->count};
-    const cuuint64_t strides[1] = {(cuuint64_t)r8_pitch(r->dim)};
-    const cuuint32_t box[2] = {(cuuint32_t)kR8Block, (cuuint32_t)rows}, step[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, r->codes, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+    const cuuint64_t dims[2] = {(cuuint64_t)r8_pitch(dim), (cuuint64_t)count};
+    const cuuint64_t strides[1] = {(cuuint64_t)r8_pitch(dim)};
+    const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)rows}, step[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? CS_OK
                : CS_E_ARG;
 }
 
 // the scale words of 128 rows as rows of 512 bytes, `chunks` consecutive tiles of 128 rows at once
-int r8_scale_map(CUtensorMap* map, const cs_rows8* r, const int chunks) {
+int r8_scale_map(CUtensorMap* map, void* base, const int dim, const int64_t count, const int chunks) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return CS_E_DEVICE;
-    const cuuint64_t words = (cuuint64_t)r8_words(r->dim);
-    const cuuint64_t dims[3] = {128, words, (cuuint64_t)((r->count + 127) / 128)};
+    const cuuint64_t words = (cuuint64_t)r8_words(dim);
+    const cuuint64_t dims[3] = {128, words, (cuuint64_t)((count + 127) / 128)};
     const cuuint64_t strides[2] = {512, words * 512};
     const cuuint32_t box[3] = {128, 1, (cuuint32_t)chunks}, step[3] = {1, 1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, r->scales, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? CS_OK
                : CS_E_ARG;
 }
 
+// what the pair kernel's extra step needs per column, rounded up to whole tiles: 16 bytes of digits, then scale words
+int64_t r8_norm_rows(const int64_t n_col) { return n_col <= 64 ? 0 : (n_col + kPairCols - 1) / kPairCols * kPairCols; }
+
 template <int WHAT, typename T>
-int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
-    CUtensorMap lane_map, col_map, lane_sf, col_sf;
-    int rc = r8_map(&lane_map, lanes, kR8Lanes);
-    if (rc) return rc;
-    rc = r8_map(&col_map, cols, kPairCols / 2);
-    if (rc) return rc;
-    rc = r8_scale_map(&lane_sf, lanes, 1);
-    if (rc) return rc;
-    rc = r8_scale_map(&col_sf, cols, 2);
-    if (rc) return rc;
-    static thread_local KernelTune tune;
-    rc = tune_kernel(rows8_pair_kernel<WHAT, T>, tune, d.dev, kPairSmem, kPairWarps * 32, nullptr);
+int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, void* work, cudaStream_t st, const DevInfo& d) {
+    using S = PairShape<WHAT>;
+    PairMaps maps = {};
+    int rc = r8_map(&maps.lane, lanes->codes, lanes->dim, lanes->count, kR8Block, kR8Lanes, true);
+    if (!rc) rc = r8_map(&maps.col, cols->codes, cols->dim, cols->count, kR8Block, kPairCols / 2, true);
+    if (!rc) rc = r8_scale_map(&maps.lane_sf, lanes->scales, lanes->dim, lanes->count, 1);
+    if (!rc) rc = r8_scale_map(&maps.col_sf, cols->scales, cols->dim, cols->count, 2);
     if (rc) return rc;
     const int64_t pairs = d.sms / 2, lane_tiles = (job.n_lane + kPairLanes - 1) / kPairLanes;
     job.col_tiles = (int)((job.n_col + kPairCols - 1) / kPairCols);
     job.col_split = 1;
-    if (WHAT == R8_COVERAGE) {
+    if (S::kNorms) {
+        const int64_t rows = r8_norm_rows(job.n_col);
+        unsigned char* digits = static_cast<unsigned char*>(work);
+        unsigned char* scales = digits + rows * 16;
+        const int64_t n_h = job.keep ? 0 : job.n_lane, most = rows > n_h ? rows : n_h;
+        rows8_norm_digits_kernel<<<r8_grid((most + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(job.col_norms, job.n_col, rows, digits, scales,
+                                                                                                 static_cast<float*>(job.out), n_h);
+        rc = check_launch();
+        if (!rc) rc = r8_map(&maps.norm, digits, 16, rows, 16, kPairCols / 2, false);
+        if (!rc) rc = r8_scale_map(&maps.norm_sf, scales, 1, rows, 2);
+        if (rc) return rc;
+        // few lane tiles: split the centres until every pair has work
         int64_t want = (pairs + lane_tiles - 1) / lane_tiles;
         want = want > job.col_tiles ? job.col_tiles : want;
         job.col_split = (int)((job.col_tiles + want - 1) / want);
     }
+    static thread_local KernelTune tune;
+    rc = tune_kernel(rows8_pair_kernel<WHAT, T>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
+    if (rc) return rc;
     job.splits = (job.col_tiles + job.col_split - 1) / job.col_split;
     job.items = lane_tiles * job.splits;
-    if (WHAT == R8_COVERAGE && !job.keep) {
-        rows8_fill_kernel<<<r8_grid((job.n_lane + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(
-            static_cast<float*>(job.out), job.n_lane, __builtin_huge_valf());
-        rc = check_launch();
-        if (rc) return rc;
-    }
     const int grid = 2 * (int)(job.items < pairs ? job.items : pairs);
-    rows8_pair_kernel<WHAT, T><<<grid, kPairWarps * 32, kPairSmem, st>>>(lane_map, col_map, lane_sf, col_sf, job);
+    rows8_pair_kernel<WHAT, T><<<grid, kPairWarps * 32, S::kSmem, st>>>(maps, job);
     return check_launch();
 }
 
 template <int NT, int WHAT, typename T>
 int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
     CUtensorMap lane_map, col_map;
-    int rc = r8_map(&lane_map, lanes, kR8Lanes);
+    int rc = r8_map(&lane_map, lanes->codes, lanes->dim, lanes->count, kR8Block, kR8Lanes, true);
     if (rc) return rc;
-    rc = r8_map(&col_map, cols, NT);
+    rc = r8_map(&col_map, cols->codes, cols->dim, cols->count, kR8Block, NT, true);
     if (rc) return rc;
     static thread_local KernelTune tune;
     rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, R8Shape<NT>::kSmem, 192, nullptr);
@@ -171,11 +178,11 @@ int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cu
 // the narrowest tile that holds all columns; pairs of SMs where 64 do not (coverage of 1M x 128 by 8192 centres:
 // 1.28 ms, with tiles of 128 x 128 on single SMs 3.11 ms)
 template <int WHAT, typename T>
-int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
+int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, void* work, cudaStream_t st, const DevInfo& d) {
     if (job.n_col <= 16) return launch_rows8_mma<16, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 32) return launch_rows8_mma<32, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 64) return launch_rows8_mma<64, WHAT, T>(lanes, cols, job, st, d);
-    return launch_rows8_pair<WHAT, T>(lanes, cols, job, st, d);
+    return launch_rows8_pair<WHAT, T>(lanes, cols, job, work, st, d);
 }
 
 R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {
@@ -259,12 +266,18 @@ int cs_rows8_products(const cs_rows8* a, const cs_rows8* b, void* out, int32_t d
     job.lane_stride = swap ? ld : 1;
     job.col_stride = swap ? 1 : ld;
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == CS_DTYPE_F32) return launch_rows8_mma<R8_PRODUCTS, float>(lanes, cols, job, st, d);
-    if (dtype == CS_DTYPE_F16) return launch_rows8_mma<R8_PRODUCTS, __half>(lanes, cols, job, st, d);
-    return launch_rows8_mma<R8_PRODUCTS, __nv_bfloat16>(lanes, cols, job, st, d);
+    if (dtype == CS_DTYPE_F32) return launch_rows8_mma<R8_PRODUCTS, float>(lanes, cols, job, nullptr, st, d);
+    if (dtype == CS_DTYPE_F16) return launch_rows8_mma<R8_PRODUCTS, __half>(lanes, cols, job, nullptr, st, d);
+    return launch_rows8_mma<R8_PRODUCTS, __nv_bfloat16>(lanes, cols, job, nullptr, st, d);
 }
 
-int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int32_t keep, cs_stream stream) {
+int64_t cs_rows8_coverage_bytes(int64_t n_centres) {
+    if (n_centres < 0) return CS_E_ARG;
+    const int64_t rows = r8_norm_rows(n_centres);
+    return rows * 16 + (rows + 127) / 128 * 512;
+}
+
+int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int32_t keep, void* work, cs_stream stream) {
     int rc = validate_rows8(a);
     if (rc) return rc;
     rc = validate_rows8(centres);
@@ -281,10 +294,12 @@ int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int3
         rows8_fill_kernel<<<r8_grid((a->count + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(h, a->count, __builtin_huge_valf());
         return check_launch();
     }
+    if (r8_norm_rows(centres->count) > 0 && !work) return CS_E_ARG;
+    if ((uintptr_t)work & 15u) return CS_E_ALIGN;
     R8Job job = r8_job(a, centres);
     job.out = h;
     job.keep = keep != 0;
-    return launch_rows8_mma<R8_COVERAGE, float>(a, centres, job, st, d);
+    return launch_rows8_mma<R8_COVERAGE, float>(a, centres, job, work, st, d);
 }
 
 }  // extern "C"

@@ -41,7 +41,8 @@ struct R8Job {
 };
 
 __device__ __forceinline__ uint64_t umma_desc(const uint32_t smem, const uint32_t stride_bytes, const uint64_t swizzle) {
-    // start >> 4, stride between groups of 8 rows >> 4, the constant 1 of this architecture, swizzle mode
+    // start >> 4, stride between the 16-byte halves of a step's codes >> 4 (1; unused with a swizzle), stride
+    // between groups of 8 rows >> 4, the constant 1 of this architecture, swizzle mode
     return (uint64_t)((smem & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(stride_bytes >> 4) << 32) | (1ull << 46) | (swizzle << 61);
 }
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, const int x, const int y, uint64_t* bar) {

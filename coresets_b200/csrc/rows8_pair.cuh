@@ -5,6 +5,13 @@
 // holds 128 rows of the lane operand and half of the column operand's rows, and each tensor core reads the
 // halves of both.  That halves what a block has to fetch for its share of the column operand.  TMEM: two
 // accumulators of 192 columns, and per stage 4 + 8 columns of scales.
+//
+// Coverage needs max_j (a.c_j - |c_j|^2 / 2) per row.  The norms come in through the tensor core as one more
+// step of 32 elements: -|c|^2 / 2 is a 24-bit number, six digits of 4 bits that e4m3 holds exactly, times
+// six powers of two that stand in the lane operand, times one exponent per column.  The readers are left with one
+// three-input maximum per two columns.  Reading the norms from shared memory instead costs 4 wavefronts per
+// 16 bytes, and that pipe then sets the pace (1M x 128 by 8192 centres: 1.28 ms; with the extra step PERF).
+//
 // The even block ("leader") issues every MMA; the full and the accumulator-free barriers are its own,
 // the stage-free and the accumulator-full barriers exist in both blocks and are reached by multicast commits.
 #ifndef CORESETS_B200_ROWS8_PAIR_CUH
@@ -13,14 +20,22 @@
 namespace {
 
 constexpr int kPairCols = 192, kPairLanes = 256;
-constexpr int kPairStages = 7, kPairReaders = 16, kPairWarps = 2 + kPairReaders;
+constexpr int kPairReaders = 16, kPairWarps = 2 + kPairReaders;
 constexpr int kPairPart = kPairCols / (kPairReaders / 4);        // columns of a reading warp
-constexpr int kPairSlots = 8;                                   // TMEM slots of scales, one per 4 blocks of a row: a slot comes round
-                                                                // after 8 stages at least, when the stage 7 back is known to be done
 constexpr int kPairA = kR8Lanes * kR8Block, kPairB = kPairCols / 2 * kR8Block;
 constexpr int kPairSf = 512 + 1024;                              // scale words of 128 lanes, and of the columns' two chunks of 128
-constexpr int kPairStage = (kPairA + kPairB + kPairSf + 1023) & ~1023;
-constexpr int kPairSmem = kPairStages * kPairStage + 1024;
+constexpr int kPairNormB = kPairCols / 2 * 16, kPairNormSf = 1024;          // digits of the norms, and their exponents
+template <int WHAT> struct PairShape {
+    static constexpr bool kNorms = WHAT == R8_COVERAGE;
+    static constexpr int kStages = kNorms ? 6 : 7;
+    static constexpr int kFirst = kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0);   // behind the codes of a stage; 16 zero bytes end it
+    static constexpr int kStage = (kPairA + kPairB + kFirst + 1023) & ~1023;
+    static constexpr int kSmem = kStages * kStage + 1024;
+    // TMEM columns of scales, one slot per 4 blocks of a row.  A slot comes round after kStages stages at
+    // least: the MMAs that read it are known to be done, since the stage itself was free to be filled again.
+    static constexpr int kSlot = kNorms ? 20 : 12;
+};
+static_assert(2 * kPairCols + 6 * 20 + 4 <= 512 && 2 * kPairCols + 7 * 12 <= 512, "TMEM columns");
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -57,18 +72,9 @@ __device__ __forceinline__ void pair_mma(const uint32_t acc, const uint64_t a, c
                  "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p; }"
                  ::"r"(acc), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"((unsigned)add) : "memory");
 }
-// two at a time: (a, b) * (s, s) + (c, d)
-__device__ __forceinline__ float2 fma2(const float a, const float b, const float s, const float2 c) {
-    float2 r;
-    asm("{ .reg .b64 x, y, z;\n mov.b64 x, {%2, %3}; mov.b64 y, {%4, %4}; mov.b64 z, {%5, %6};\n"
-        "fma.rn.ftz.f32x2 x, x, y, z; mov.b64 {%0, %1}, x; }"
-        : "=f"(r.x), "=f"(r.y) : "f"(a), "f"(b), "f"(s), "f"(c.x), "f"(c.y));
-    return r;
-}
-
-__device__ __forceinline__ float min3(const float a, const float b, const float c) {
+__device__ __forceinline__ float max3(const float a, const float b, const float c) {
     float r;
-    asm("min.ftz.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.ftz.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 // 48 columns at once: both loads in flight before the wait
@@ -86,6 +92,25 @@ __device__ __forceinline__ void tc_load48(const uint32_t tmem, unsigned (&u)[48]
                  : "r"(tmem), "r"(tmem + 32) : "memory");
 }
 
+// Digits and exponents of -|c|^2 / 2 for the pair kernel, `rows` (whole tiles) of them, and h = +inf where asked.
+// |c|^2 = m 2^(E - 150) with 24 bits of m = sum_i d_i 16^i; the lane operand holds 2^-9, 2^-5, 2^-1, 2^3, 2^7, 2^7, so the
+// codes are -d_0 .. -d_4, -16 d_5 and the scale 2^(E - 142).  Below 2^-112 a norm counts as 0; NaN and infinity, and the
+// columns past the last, get the NaN scale: never the largest.
+__global__ void rows8_norm_digits_kernel(const float* __restrict__ norms, const int64_t n, const int64_t rows, unsigned char* digits,
+                                         unsigned char* scales, float* h, const int64_t n_h) {
+    const int64_t step = (int64_t)gridDim.x * blockDim.x, at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    for (int64_t i = at; i < rows; i += step) {
+        const unsigned bits = i < n ? __float_as_uint(__fadd_rn(__ldg(norms + i), 0.0f)) : 0x7fc00000u;      // (+ 0: no negative zero)
+        const unsigned e = (bits >> 23) & 255u, m = e >= 15u ? (bits & 0x7fffffu) | 0x800000u : 0u;
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        q.x = to_e4m3x2(-(float)(m & 15u), -(float)(m >> 4 & 15u)) | to_e4m3x2(-(float)(m >> 8 & 15u), -(float)(m >> 12 & 15u)) << 16;
+        q.y = to_e4m3x2(-(float)(m >> 16 & 15u), -16.0f * (float)(m >> 20 & 15u));
+        reinterpret_cast<uint4*>(digits)[i] = q;
+        *reinterpret_cast<unsigned*>(scales + r8_scale_word(i, 0, 1)) = (bits & 0x80000000u) || e == 255u ? 255u : (e >= 15u ? e - 15u : 0u);
+    }
+    for (int64_t i = at; i < n_h; i += step) h[i] = __uint_as_float(0x7f800000u);
+}
+
 struct PairSpan { int64_t lt; int c0, c1; };
 __device__ __forceinline__ PairSpan pair_span(const R8Job& job, const int64_t item) {
     PairSpan s;
@@ -95,15 +120,18 @@ __device__ __forceinline__ PairSpan pair_span(const R8Job& job, const int64_t it
     return s;
 }
 
+struct PairMaps { CUtensorMap lane, col, lane_sf, col_sf, norm, norm_sf; };
+
 template <int WHAT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairWarps * 32, 1)
-rows8_pair_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_constant__ CUtensorMap col_map,
-                  const __grid_constant__ CUtensorMap lane_sf_map, const __grid_constant__ CUtensorMap col_sf_map, const R8Job job) {
+rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
+    using S = PairShape<WHAT>;
+    constexpr int kStages = S::kStages;
     extern __shared__ unsigned char s_raw[];
-    __shared__ uint64_t s_full[kPairStages], s_empty[kPairStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_word;
-    __shared__ __align__(16) float s_norm[kPairReaders][kPairPart];
+    __shared__ __align__(1024) unsigned char s_power[S::kNorms ? 4096 + 512 : 16];      // the lane operand of the norms' step, and its scales
     volatile int* s_abort = &s_abort_word;
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
 
@@ -113,9 +141,17 @@ rows8_pair_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_con
     const int kblocks = (job.D + kR8Block - 1) / kR8Block;
     if (threadIdx.x == 0) {
         s_abort_word = 0;
-        for (int i = 0; i < kPairStages; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 1); }
+        for (int i = 0; i < kStages; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 2 * kPairReaders); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (S::kNorms) {
+        // 128 equal rows of 32 codes without a swizzle: 16 bytes of a row, 8 rows a group; the second 16 are 0
+        for (int i = threadIdx.x; i < (4096 + 512) / 4; i += blockDim.x)
+            reinterpret_cast<unsigned*>(s_power)[i] = i >= 1024 ? 0x7f7f7f7fu : (i < 512 && (i & 3) == 0 ? 0x50301001u : (i < 512 && (i & 3) == 1 ? 0x7070u : 0u));
+        if (threadIdx.x < kStages * 4)
+            *reinterpret_cast<unsigned*>(tiles + (threadIdx.x >> 2) * S::kStage + kPairA + kPairB + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
@@ -137,33 +173,39 @@ rows8_pair_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_con
             const int row = (int)(sp.lt * kPairLanes) + (int)rank * kR8Lanes;
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct)
                 for (int kb = 0; kb < kblocks; ++kb, ++n) {
-                    if (n >= kPairStages && !r8_wait_warp(&s_empty[st], phase ^ 1u, s_abort)) { ok = false; break; }
-                    const uint32_t a = smem_u32(tiles + st * kPairStage), bar = leader_addr(&s_full[st]);
+                    if (n >= kStages && !r8_wait_warp(&s_empty[st], phase ^ 1u, s_abort)) { ok = false; break; }
+                    const uint32_t a = smem_u32(tiles + st * S::kStage), bar = leader_addr(&s_full[st]);
                     const bool scales = (kb & 3) == 0;
                     if (elect_one()) {
-                        if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (kPairA + kPairB + (scales ? kPairSf : 0)));
-                        pair_tile(a, &lane_map, kb * kR8Block, row, bar);
-                        pair_tile(a + kPairA, &col_map, kb * kR8Block, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
+                        if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (kPairA + kPairB + (scales ? kPairSf : 0) + (S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0)));
+                        pair_tile(a, &maps.lane, kb * kR8Block, row, bar);
+                        pair_tile(a + kPairA, &maps.col, kb * kR8Block, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
                         if (scales) {
-                            pair_scales(a + kPairA + kPairB, &lane_sf_map, kb >> 2, row >> 7, bar);
-                            pair_scales(a + kPairA + kPairB + 512, &col_sf_map, kb >> 2, ct * kPairCols >> 7, bar);
+                            pair_scales(a + kPairA + kPairB, &maps.lane_sf, kb >> 2, row >> 7, bar);
+                            pair_scales(a + kPairA + kPairB + 512, &maps.col_sf, kb >> 2, ct * kPairCols >> 7, bar);
+                        }
+                        if (S::kNorms && kb == 0) {
+                            pair_tile(a + kPairA + kPairB + kPairSf + kPairNormSf, &maps.norm, 0, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
+                            pair_scales(a + kPairA + kPairB + kPairSf, &maps.norm_sf, 0, ct * kPairCols >> 7, bar);
                         }
                     }
                     __syncwarp();
-                    if (++st == kPairStages) { st = 0; phase ^= 1u; }
+                    if (++st == kStages) { st = 0; phase ^= 1u; }
                 }
         }
         // no copy may be in flight when the pair leaves (they all are complete unless a role gave up)
         if (!ok && rank == 0)
-            for (uint32_t k = n > kPairStages ? n - kPairStages : 0; k < n; ++k)
-                for (int it = 0; it < (1 << 16) && !mbar_try(&s_full[k % kPairStages], (k / kPairStages) & 1u); ++it) {}
+            for (uint32_t k = n > kStages ? n - kStages : 0; k < n; ++k)
+                for (int it = 0; it < (1 << 16) && !mbar_try(&s_full[k % kStages], (k / kStages) & 1u); ++it) {}
     } else if (warp == 1) {
         if (rank == 0) {
             uint32_t st = 0, phase = 0, slot = 0;
             uint32_t n = 0, t = 0;
             bool ok = true;
             constexpr uint32_t kIdesc = ((uint32_t)(kPairCols >> 3) << 17) | (1u << 23) | ((uint32_t)(kPairLanes >> 4) << 24);
-            const uint32_t base = smem_u32(tiles);
+            const uint32_t base = smem_u32(tiles), power = smem_u32(s_power), sf_power = tmem + kSf + kStages * S::kSlot;
+            if (S::kNorms && elect_one()) pair_copy_scales(sf_power, umma_desc(power + 4096, 128, 0));
+            __syncwarp();
             for (int64_t item = first; item < job.items && ok; item += stride) {
                 const PairSpan sp = pair_span(job, item);
                 for (int ct = sp.c0; ct < sp.c1 && ok; ++ct, ++t) {
@@ -176,10 +218,10 @@ rows8_pair_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_con
                     for (int kb = 0; kb < kblocks; ++kb, ++n) {
                         if (!r8_wait_warp(&s_full[st], phase, s_abort)) { ok = false; break; }
                         tc_fence_after();
-                        if ((kb & 3) == 0 && ++slot == kPairSlots) slot = 0;
+                        if ((kb & 3) == 0 && ++slot == kStages) slot = 0;
                         if (elect_one()) {
-                            const uint32_t a = base + st * kPairStage, b = a + kPairA, sf = b + kPairB;
-                            const uint32_t sfa = tmem + kSf + slot * 12, sfb = sfa + 4;
+                            const uint32_t a = base + st * S::kStage, b = a + kPairA, sf = b + kPairB, norm = sf + kPairSf;
+                            const uint32_t sfa = tmem + kSf + slot * S::kSlot, sfb = sfa + 4;
                             if ((kb & 3) == 0) {
                                 pair_copy_scales(sfa, umma_desc(sf, 128, 0));
                                 pair_copy_scales(sfb, umma_desc(sf + 512, 128, 0));
@@ -195,45 +237,38 @@ rows8_pair_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_con
                                 const int steps = (left + 31) >> 5;
                                 for (int k = 0; k < steps; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
                             }
+                            if (S::kNorms && kb == 0) {
+                                // 16 of the step's 32 codes count (the lane operand's others are 0): as the second
+                                // 16 of a row the descriptor names the next row's digits, then the zero bytes
+                                pair_copy_scales(sfb + 8, umma_desc(norm, 128, 0));
+                                pair_copy_scales(sfb + 12, umma_desc(norm + 512, 128, 0));
+                                pair_mma(acc, umma_desc(power, 128, 0) + (127ull << 16), umma_desc(norm + kPairNormSf, 128, 0), kIdesc, sf_power,
+                                         sfb + 8 + sub, true);
+                            }
                             pair_commit(&s_empty[st]);
                             if (kb == kblocks - 1) pair_commit(&s_acc_full[buf]);
                         }
                         __syncwarp();
-                        if (++st == kPairStages) { st = 0; phase ^= 1u; }
+                        if (++st == kStages) { st = 0; phase ^= 1u; }
                     }
                 }
             }
             if (!ok)
-                for (uint32_t k = n > kPairStages ? n - kPairStages : 0; k < n; ++k)
-                    for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % kPairStages], (k / kPairStages) & 1u); ++it) {}
+                for (uint32_t k = n > kStages ? n - kStages : 0; k < n; ++k)
+                    for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % kStages], (k / kStages) & 1u); ++it) {}
         }
     } else {
         const int quad = warp & 3, part = (warp - 2) >> 2;
-        float* norm = s_norm[warp - 2];
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + part * kPairPart;
-        const float inf = __uint_as_float(0x7f800000u);
+        const float low = __uint_as_float(0xff800000u);
         uint32_t t = 0;
         bool ok = true;
         for (int64_t item = first; item < job.items && ok; item += stride) {
             const PairSpan sp = pair_span(job, item);
             const int64_t row = sp.lt * kPairLanes + rank * kR8Lanes + quad * 32 + lane;
-            float best[4] = {inf, inf, inf, inf};
-            // the centres' norms of the next tile, one tile ahead; past the last centre nothing is near
-            float2 ahead;
-            const auto fetch = [&](const int ct) {
-                const int64_t col = (int64_t)ct * kPairCols + part * kPairPart + 2 * lane;
-                ahead.x = 2 * lane < kPairPart && col < job.n_col ? __ldg(job.col_norms + col) : inf;
-                ahead.y = 2 * lane < kPairPart && col + 1 < job.n_col ? __ldg(job.col_norms + col + 1) : inf;
-            };
-            if (WHAT == R8_COVERAGE) fetch(sp.c0);
+            float best[4] = {low, low, low, low};
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct, ++t) {
                 const uint32_t buf = t & 1u;
-                if (WHAT == R8_COVERAGE) {
-                    __syncwarp();
-                    if (2 * lane < kPairPart) *reinterpret_cast<float2*>(norm + 2 * lane) = ahead;
-                    __syncwarp();
-                    if (ct + 1 < sp.c1) fetch(ct + 1);
-                }
                 ok = r8_wait_warp(&s_acc_full[buf], (t >> 1) & 1u, s_abort);
                 if (!ok) break;
                 tc_fence_after();
@@ -259,17 +294,13 @@ rows8_pair_kernel(const __grid_constant__ CUtensorMap lane_map, const __grid_con
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < kPairPart; j += 4) {
-                        const float4 n4 = *reinterpret_cast<const float4*>(norm + j);
-                        const float2 p = fma2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]), -2.0f, make_float2(n4.x, n4.y));
-                        const float2 q = fma2(__uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]), -2.0f, make_float2(n4.z, n4.w));
-                        best[(j >> 1) & 3] = min3(best[(j >> 1) & 3], p.x, p.y);
-                        best[((j >> 1) + 1) & 3] = min3(best[((j >> 1) + 1) & 3], q.x, q.y);
-                    }
+                    for (int j = 0; j < kPairPart; j += 2)
+                        best[(j >> 1) & 3] = max3(best[(j >> 1) & 3], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                 }
             }
             if (WHAT == R8_COVERAGE && ok && row < job.n_lane) {
-                const float d = __fadd_rn(__ldg(job.lane_norms + row), fminf(fminf(best[0], best[1]), fminf(best[2], best[3])));
+                // |a - c|^2 = |a|^2 - 2 (a.c - |c|^2 / 2)
+                const float d = __fmaf_rn(-2.0f, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])), __ldg(job.lane_norms + row));
                 if (d == d)      // h holds +inf or what it had: a NaN leaves that; max(d, 0) orders like its bits
                     atomicMin(reinterpret_cast<int*>(job.out) + row, __float_as_int(fmaxf(d, 0.0f)));
             }

@@ -12,7 +12,7 @@ float32.  The rounding to e4m3 is off by at most 2^-4 of an element, or 2^-10 of
 the rows as stored, with float32 sums.
 
 Every call is enqueued on the current stream of the store's device, allocates nothing but its result (and a
-contiguous copy of an input whose columns are strided), synchronises with nothing and can be captured into
+contiguous copy of an input whose columns are strided, and 20 bytes of scratch per centre), synchronises with nothing and can be captured into
 a CUDA graph.
 """
 from __future__ import annotations
@@ -280,8 +280,11 @@ def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
     else:
         h = torch.empty(n, dtype=torch.float32, device=store.device)
     if n:
+        native = _native.get_native()
+        size = native.lib.cs_rows8_coverage_bytes(centres.count)
+        work = torch.empty(size, dtype=torch.uint8, device=store.device) if size else None
         with _on(store.device) as stream:
-            _native.get_native().rows8_coverage(store._c, centres._c, h.data_ptr(), int(keep), stream)
+            native.rows8_coverage(store._c, centres._c, h.data_ptr(), int(keep), work.data_ptr() if size else None, stream)
     return h
 
 

@@ -73,7 +73,7 @@ def test_c_abi_refusals(lib):
         assert lib.cs_rows8_read(r(bad), p, 1, p, 0, 64, None) == code
         assert lib.cs_rows8_take(r(bad), p, 1, r(good), 0, None) == code
         assert lib.cs_rows8_products(r(good), r(bad), p, 0, 64, None) == code
-        assert lib.cs_rows8_coverage(r(bad), r(good), p, 0, None) == code
+        assert lib.cs_rows8_coverage(r(bad), r(good), p, 0, p, None) == code
     assert lib.cs_rows8_write(None, p, 0, 1, 64, 0, None) == ARG
     for args in ((p, 3, 1, 64, 0), (p, 0, -1, 64, 0), (None, 0, 1, 64, 0), (p, 0, 2, 63, 0), (p, 0, 1, 64, 100), (p, 0, 51, 64, 50), (p, 0, 1, 64, -1),
                  (p, 0, 2 ** 62, 64, 2)):
@@ -86,11 +86,13 @@ def test_c_abi_refusals(lib):
     assert lib.cs_rows8_products(r(good), r(other), p, 0, 64, None) == ARG
     assert lib.cs_rows8_products(r(good), r(good), p, 0, 49, None) == ARG
     assert lib.cs_rows8_products(r(good), r(good), p + 2, 0, 50, None) == ALIGN
-    assert lib.cs_rows8_coverage(r(good), r(good), None, 0, None) == ARG
-    assert lib.cs_rows8_coverage(r(good), r(good), p + 2, 0, None) == ALIGN
+    assert lib.cs_rows8_coverage(r(good), r(good), None, 0, None, None) == ARG
+    assert lib.cs_rows8_coverage(r(good), r(good), p + 2, 0, None, None) == ALIGN
+    many = _store(codes=40960, scales=81920, count=100)
+    assert lib.cs_rows8_coverage_bytes(64) == 0 and lib.cs_rows8_coverage_bytes(100) >= 20 * 100 and lib.cs_rows8_coverage_bytes(-1) == ARG
     # nothing to do
     none = _store(count=0)
     assert lib.cs_rows8_write(r(good), None, 0, 0, 64, 100, None) == 0
     assert lib.cs_rows8_read(r(none), None, 0, None, 0, 64, None) == 0
     assert lib.cs_rows8_products(r(none), r(good), None, 0, 50, None) == 0
-    assert lib.cs_rows8_coverage(r(none), r(good), None, 0, None) == 0
+    assert lib.cs_rows8_coverage(r(none), r(good), None, 0, None, None) == 0
