@@ -36,6 +36,7 @@ struct R8Job {
     int64_t items;                                  // lane tiles * splits
     void* out;                                      // products: P; coverage: h
     int64_t lane_stride, col_stride;                // products, in elements
+    int bulk_out;                                   // products: out takes bulk stores
     int keep;                                       // coverage: min with what h holds
     int* status;
 };

@@ -25,17 +25,18 @@ constexpr int kPairPart = kPairCols / (kPairReaders / 4);        // columns of a
 constexpr int kPairA = kR8Lanes * kR8Block, kPairB = kPairCols / 2 * kR8Block;
 constexpr int kPairSf = 512 + 1024;                              // scale words of 128 lanes, and of the columns' two chunks of 128
 constexpr int kPairNormB = kPairCols / 2 * 16, kPairNormSf = 1024;          // digits of the norms, and their exponents
-template <int WHAT> struct PairShape {
+template <int WHAT, typename T> struct PairShape {
     static constexpr bool kNorms = WHAT == R8_COVERAGE;
-    static constexpr int kStages = kNorms ? 6 : 7;
-    static constexpr int kFirst = kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0);   // behind the codes of a stage; 16 zero bytes end it
-    static constexpr int kStage = (kPairA + kPairB + kFirst + 1023) & ~1023;
-    static constexpr int kSmem = kStages * kStage + 1024;
+    static constexpr int kOut = kNorms ? 0 : kPairReaders * kPairPart * 32 * (int)sizeof(T);     // a reading warp's share of a tile of products
+    static constexpr int kStages = !kNorms && sizeof(T) == 4 ? 4 : 6;
+    static constexpr int kTile = kPairA + kPairB;                              // codes of a stage
+    static constexpr int kFirst = (kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0) + 127) & ~127;    // what else a stage may bring in (digits end with 16 zero bytes)
+    static constexpr int kSmem = kStages * (kTile + kFirst) + kOut + 1024;
     // TMEM columns of scales, one slot per 4 blocks of a row.  A slot comes round after kStages stages at
     // least: the MMAs that read it are known to be done, since the stage itself was free to be filled again.
     static constexpr int kSlot = kNorms ? 20 : 12;
 };
-static_assert(2 * kPairCols + 6 * 20 + 4 <= 512 && 2 * kPairCols + 7 * 12 <= 512, "TMEM columns");
+static_assert(2 * kPairCols + 6 * 20 + 4 <= 512 && 2 * kPairCols + 6 * 12 <= 512, "TMEM columns");
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -120,12 +121,12 @@ __device__ __forceinline__ PairSpan pair_span(const R8Job& job, const int64_t it
     return s;
 }
 
-struct PairMaps { CUtensorMap lane, col, lane_sf, col_sf, norm, norm_sf; };
+struct PairMaps { CUtensorMap lane, col, lane_sf, col_sf, norm, norm_sf, out; };
 
 template <int WHAT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairWarps * 32, 1)
 rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
-    using S = PairShape<WHAT>;
+    using S = PairShape<WHAT, T>;
     constexpr int kStages = S::kStages;
     extern __shared__ unsigned char s_raw[];
     __shared__ uint64_t s_full[kStages], s_empty[kStages], s_acc_full[2], s_acc_empty[2];
@@ -150,7 +151,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
         for (int i = threadIdx.x; i < (4096 + 512) / 4; i += blockDim.x)
             reinterpret_cast<unsigned*>(s_power)[i] = i >= 1024 ? 0x7f7f7f7fu : (i < 512 && (i & 3) == 0 ? 0x50301001u : (i < 512 && (i & 3) == 1 ? 0x7070u : 0u));
         if (threadIdx.x < kStages * 4)
-            *reinterpret_cast<unsigned*>(tiles + (threadIdx.x >> 2) * S::kStage + kPairA + kPairB + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
+            *reinterpret_cast<unsigned*>(tiles + kStages * S::kTile + (threadIdx.x >> 2) * S::kFirst + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
@@ -174,19 +175,19 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct)
                 for (int kb = 0; kb < kblocks; ++kb, ++n) {
                     if (n >= kStages && !r8_wait_warp(&s_empty[st], phase ^ 1u, s_abort)) { ok = false; break; }
-                    const uint32_t a = smem_u32(tiles + st * S::kStage), bar = leader_addr(&s_full[st]);
+                    const uint32_t a = smem_u32(tiles + st * S::kTile), sf = smem_u32(tiles + kStages * S::kTile + st * S::kFirst), bar = leader_addr(&s_full[st]);
                     const bool scales = (kb & 3) == 0;
                     if (elect_one()) {
                         if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (kPairA + kPairB + (scales ? kPairSf : 0) + (S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0)));
                         pair_tile(a, &maps.lane, kb * kR8Block, row, bar);
                         pair_tile(a + kPairA, &maps.col, kb * kR8Block, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
                         if (scales) {
-                            pair_scales(a + kPairA + kPairB, &maps.lane_sf, kb >> 2, row >> 7, bar);
-                            pair_scales(a + kPairA + kPairB + 512, &maps.col_sf, kb >> 2, ct * kPairCols >> 7, bar);
+                            pair_scales(sf, &maps.lane_sf, kb >> 2, row >> 7, bar);
+                            pair_scales(sf + 512, &maps.col_sf, kb >> 2, ct * kPairCols >> 7, bar);
                         }
                         if (S::kNorms && kb == 0) {
-                            pair_tile(a + kPairA + kPairB + kPairSf + kPairNormSf, &maps.norm, 0, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
-                            pair_scales(a + kPairA + kPairB + kPairSf, &maps.norm_sf, 0, ct * kPairCols >> 7, bar);
+                            pair_tile(sf + kPairSf + kPairNormSf, &maps.norm, 0, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
+                            pair_scales(sf + kPairSf, &maps.norm_sf, 0, ct * kPairCols >> 7, bar);
                         }
                     }
                     __syncwarp();
@@ -220,7 +221,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                         tc_fence_after();
                         if ((kb & 3) == 0 && ++slot == kStages) slot = 0;
                         if (elect_one()) {
-                            const uint32_t a = base + st * S::kStage, b = a + kPairA, sf = b + kPairB, norm = sf + kPairSf;
+                            const uint32_t a = base + st * S::kTile, b = a + kPairA, sf = base + kStages * S::kTile + st * S::kFirst, norm = sf + kPairSf;
                             const uint32_t sfa = tmem + kSf + slot * S::kSlot, sfb = sfa + 4;
                             if ((kb & 3) == 0) {
                                 pair_copy_scales(sfa, umma_desc(sf, 128, 0));
@@ -282,8 +283,23 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(&s_acc_empty[buf])) : "memory");
                 if (WHAT == R8_PRODUCTS) {
                     const int64_t col = (int64_t)ct * kPairCols + part * kPairPart;
-                    T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride + col * job.col_stride;
-                    if (row < job.n_lane) {
+                    if (job.bulk_out) {
+                        // 48 columns x 32 lanes through shared memory, one bulk store for the warp (it leaves out what lies
+                        // past the last lane or column)
+                        T* mine = reinterpret_cast<T*>(tiles + kStages * (S::kTile + S::kFirst)) + (warp - 2) * (kPairPart * 32);
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < kPairPart; ++j) r8_narrow(mine[j * 32 + lane], __uint_as_float(v[j]));
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0 && row < job.n_lane && col < job.n_col) {
+                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                                         ::"l"(&maps.out), "r"((int)row), "r"((int)col), "r"(smem_u32(mine)) : "memory");
+                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        }
+                    } else if (row < job.n_lane) {
+                        T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride + col * job.col_stride;
 #pragma unroll
                         for (int j = 0; j < kPairPart; ++j)
                             if (col + j < job.n_col) {
@@ -305,6 +321,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     atomicMin(reinterpret_cast<int*>(job.out) + row, __float_as_int(fmaxf(d, 0.0f)));
             }
         }
+        if (WHAT == R8_PRODUCTS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     tc_fence_before();
