@@ -18,12 +18,12 @@ int r8_grid(const int64_t groups, const DevInfo& d) {
     return (int)(groups < 1 ? 1 : (groups < cap ? groups : cap));
 }
 
-template <typename T, int G>
+template <typename T, int G, int U = 1>
 int launch_rows8_write(const cs_rows8* r, const T* X, int64_t n, int64_t ld, int64_t start, cudaStream_t st, const DevInfo& d) {
     const bool vec = ((uintptr_t)X & 15u) == 0 && (ld * sizeof(T)) % 16 == 0 && (r->dim & 7) == 0;
     const int grid = r8_grid((n + kThreads / G - 1) / (kThreads / G), d);
-    if (vec) rows8_write_kernel<T, G, true><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
-    else rows8_write_kernel<T, G, false><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    if (vec) rows8_write_kernel<T, G, U, true><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    else rows8_write_kernel<T, G, U, false><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
     return check_launch();
 }
 template <typename T>
@@ -34,7 +34,8 @@ int launch_rows8_write(const cs_rows8* r, const void* X, int64_t n, int64_t ld, 
     if (r->dim <= 16) return launch_rows8_write<T, 2>(r, x, n, ld, start, st, d);
     if (r->dim <= 32) return launch_rows8_write<T, 4>(r, x, n, ld, start, st, d);
     if (r->dim <= 64) return launch_rows8_write<T, 8>(r, x, n, ld, start, st, d);
-    return launch_rows8_write<T, 16>(r, x, n, ld, start, st, d);
+    if (r->dim <= 128) return launch_rows8_write<T, 16>(r, x, n, ld, start, st, d);
+    return launch_rows8_write<T, 16, 2>(r, x, n, ld, start, st, d);
 }
 
 template <typename T, int G>

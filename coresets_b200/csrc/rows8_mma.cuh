@@ -119,6 +119,8 @@ template <int NT> struct R8Shape {
     static constexpr int kTileA = kR8Lanes * kR8Block, kTileB = NT * kR8Block;
     static constexpr int kStage = kTileA + kTileB + 1024;              // two tiles, two scale words of 128 rows
     static constexpr int kStages = 8;
+    static constexpr int kAcc = 256 / (NT < 32 ? 32 : NT);             // accumulators: 8, 8, 4; the way from a tile's last MMA to its
+                                                                       // free accumulator is much longer than its few MMAs
     static constexpr int kSmem = kStages * kStage + 1024;              // slack to align the tiles to 1 KB
 };
 
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
     using S = R8Shape<NT>;
     constexpr int NC = NT < 32 ? NT : 32;                              // columns read back at a time
     extern __shared__ unsigned char s_raw[];
-    __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_acc_full[2], s_acc_empty[2];
+    __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_acc_full[S::kAcc], s_acc_empty[S::kAcc];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_word;
     __shared__ __align__(16) float s_norm[4][NT < 32 ? 32 : NT];          // a copy per reading warp: no barrier between them
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
     if (threadIdx.x == 0) {
         s_abort_word = 0;
         for (int i = 0; i < S::kStages; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 128); }
+        for (int i = 0; i < S::kAcc; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -190,9 +192,9 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
             const int c0 = (int)(item % job.splits) * job.col_split;
             const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
             for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
-                const uint32_t buf = t & 1u, round = t >> 1;
+                const uint32_t buf = t % S::kAcc, round = t / S::kAcc;
                 if (round > 0 && !r8_wait_warp(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
-                const uint32_t acc = tmem + buf * 128;
+                const uint32_t acc = tmem + buf * (256 / S::kAcc);
                 for (int kb = 0; kb < kblocks; ++kb, ++n) {
                     const uint32_t st = n % S::kStages;
                     if (!r8_wait_warp(&s_full[st], (n / S::kStages) & 1u, s_abort)) { ok = false; break; }
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
             const int64_t row = lt * kR8Lanes + quad * 32 + lane;
             float best = __uint_as_float(0x7f800000u);
             for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
-                const uint32_t buf = t & 1u;
+                const uint32_t buf = t % S::kAcc;
                 if (WHAT == R8_COVERAGE) {
                     // norms of the tile's centres; a column past the last centre can never be the nearest
                     __syncwarp();
@@ -240,12 +242,12 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
                     }
                     __syncwarp();
                 }
-                ok = r8_wait_warp(&s_acc_full[buf], (t >> 1) & 1u, s_abort);
+                ok = r8_wait_warp(&s_acc_full[buf], (t / S::kAcc) & 1u, s_abort);
                 if (!ok) break;
                 tc_fence_after();
                 for (int c = 0; c < NT; c += NC) {
                     unsigned v[NC];
-                    tc_load(lanes + buf * 128 + c, v);
+                    tc_load(lanes + buf * (256 / S::kAcc) + c, v);
                     if (WHAT == R8_PRODUCTS) {
                         const int64_t col = (int64_t)ct * NT + c;
                         T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride + col * job.col_stride;
@@ -264,7 +266,8 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(&s_acc_empty[buf]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_acc_empty[buf]);
             }
             if (WHAT == R8_COVERAGE && ok && row < job.n_lane) {
                 // |a - c|^2 = |a|^2 + (|c|^2 - 2 a.c); a NaN never lowers h, rounding never makes it negative

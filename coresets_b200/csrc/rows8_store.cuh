@@ -67,8 +67,8 @@ __device__ __forceinline__ void r8_load8(const T* p, float (&x)[8]) {
 }
 
 // G lanes own a row (8 consecutive elements a lane and block); G < 16 serves rows of one block and 8 G
-// elements at most.  VEC: 16-byte loads (base and row stride 16-byte aligned, D a multiple of 8).
-template <typename T, int G, bool VEC>
+// elements at most.  U blocks are loaded before the first is worked on.  VEC: 16-byte loads (base and row stride 16-byte aligned, D a multiple of 8).
+template <typename T, int G, int U, bool VEC>
 __global__ void __launch_bounds__(kThreads) rows8_write_kernel(const cs_rows8 r, const T* __restrict__ X, const int64_t n,
                                                                const int64_t ld, const int64_t start) {
     const int D = r.dim, blocks = (D + kR8Block - 1) / kR8Block, words = r8_words(D);
@@ -84,50 +84,58 @@ __global__ void __launch_bounds__(kThreads) rows8_write_kernel(const cs_rows8 r,
         unsigned char* dst = reinterpret_cast<unsigned char*>(r.codes) + row * pitch;
         float norm = 0.0f;
         unsigned word = 0u;
-        for (int b = 0; b < blocks; ++b) {
-            const int c = b * kR8Block + 8 * sub;
-            float x[8];
+        for (int b0 = 0; b0 < blocks; b0 += U) {
+            float x[U][8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-            if (VEC) {
-                if (live && c < D) r8_load8(src + c, x);
-            } else {
+            for (int u = 0; u < U; ++u) {
+                const int c = (b0 + u) * kR8Block + 8 * sub;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (live && c + k < D) x[k] = r8_widen(src[c + k]);
-            }
-            unsigned top = 0u;             // magnitudes of finite numbers order like their bits
+                for (int k = 0; k < 8; ++k) x[u][k] = 0.0f;
+                if (VEC) {
+                    if (live && c < D) r8_load8(src + c, x[u]);
+                } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const unsigned m = __float_as_uint(x[k]) & 0x7fffffffu;
-                if (m >= 0x7f800000u) x[k] = __uint_as_float(0x7fc00000u);
-                else top = m > top ? m : top;
+                    for (int k = 0; k < 8; ++k)
+                        if (live && c + k < D) x[u][k] = r8_widen(src[c + k]);
+                }
             }
 #pragma unroll
-            for (int off = G / 2; off > 0; off >>= 1) {
-                const unsigned o = __shfl_xor_sync(kFull, top, off);
-                top = o > top ? o : top;
-            }
-            // amax = m * 2^E with 1 <= m < 2; 448 = 1.75 * 2^8
-            int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-            e = e < kR8MinExp ? kR8MinExp : e;
-            const float inv = __uint_as_float((unsigned)(127 - e) << 23), scale = __uint_as_float((unsigned)(127 + e) << 23);
-            unsigned q[4];
-            float sum = 0.0f;
+            for (int u = 0; u < U; ++u) {
+                const int b = b0 + u, c = b * kR8Block + 8 * sub;
+                if (U > 1 && b >= blocks) break;
+                unsigned top = 0u;         // magnitudes of finite numbers order like their bits
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                q[k] = to_e4m3x2(mul_keep(x[2 * k], inv), mul_keep(x[2 * k + 1], inv));
-                const float2 v = from_e4m3x2(q[k]);
-                sum = __fmaf_rn(v.x, v.x, sum);
-                sum = __fmaf_rn(v.y, v.y, sum);
-            }
-            norm = __fadd_rn(norm, __fmul_rn(__fmul_rn(sum, scale), scale));
-            if (live && c < pitch) *reinterpret_cast<uint2*>(dst + c) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-            word |= (unsigned)(e + 127) << (8 * (b & 3));
-            if ((b & 3) == 3 || b == blocks - 1) {
-                if (live && sub == 0)
-                    *reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(r.scales) + r8_scale_word(row, b >> 2, words)) = word;
-                word = 0u;
+                for (int k = 0; k < 8; ++k) {
+                    const unsigned m = __float_as_uint(x[u][k]) & 0x7fffffffu;
+                    if (m >= 0x7f800000u) x[u][k] = __uint_as_float(0x7fc00000u);
+                    else top = m > top ? m : top;
+                }
+#pragma unroll
+                for (int off = G / 2; off > 0; off >>= 1) {
+                    const unsigned o = __shfl_xor_sync(kFull, top, off);
+                    top = o > top ? o : top;
+                }
+                // amax = m * 2^E with 1 <= m < 2; 448 = 1.75 * 2^8
+                int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+                e = e < kR8MinExp ? kR8MinExp : e;
+                const float inv = __uint_as_float((unsigned)(127 - e) << 23), scale = __uint_as_float((unsigned)(127 + e) << 23);
+                unsigned q[4];
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    q[k] = to_e4m3x2(mul_keep(x[u][2 * k], inv), mul_keep(x[u][2 * k + 1], inv));
+                    const float2 v = from_e4m3x2(q[k]);
+                    sum = __fmaf_rn(v.x, v.x, sum);
+                    sum = __fmaf_rn(v.y, v.y, sum);
+                }
+                norm = __fadd_rn(norm, __fmul_rn(__fmul_rn(sum, scale), scale));
+                if (live && c < pitch) *reinterpret_cast<uint2*>(dst + c) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+                word |= (unsigned)(e + 127) << (8 * (b & 3));
+                if ((b & 3) == 3 || b == blocks - 1) {
+                    if (live && sub == 0)
+                        *reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(r.scales) + r8_scale_word(row, b >> 2, words)) = word;
+                    word = 0u;
+                }
             }
         }
 #pragma unroll
