@@ -307,22 +307,6 @@ class Native:
     def fps_step_cells(self, s: CsState, c: CsCells, stream: int) -> None:
         self._check(self.lib.cs_fps_step_cells(ctypes.byref(s), ctypes.byref(c), stream), "cs_fps_step_cells")
 
-    def rows8_write(self, r: CsRows8, X: int, dtype: int, n: int, ld: int, start: int, stream: int) -> None:
-        self._check(self.lib.cs_rows8_write(ctypes.byref(r), X, dtype, n, ld, start, stream), "cs_rows8_write")
-
-    def rows8_read(self, r: CsRows8, rows: Optional[int], m: int, out: int, dtype: int, ld: int, stream: int) -> None:
-        self._check(self.lib.cs_rows8_read(ctypes.byref(r), rows, m, out, dtype, ld, stream), "cs_rows8_read")
-
-    def rows8_take(self, src: CsRows8, rows: int, m: int, dst: CsRows8, start: int, stream: int) -> None:
-        self._check(self.lib.cs_rows8_take(ctypes.byref(src), rows, m, ctypes.byref(dst), start, stream), "cs_rows8_take")
-
-    def rows8_products(self, a: CsRows8, b: CsRows8, out: int, dtype: int, ld: int, stream: int) -> None:
-        self._check(self.lib.cs_rows8_products(ctypes.byref(a), ctypes.byref(b), out, dtype, ld, stream), "cs_rows8_products")
-
-    def rows8_coverage(self, a: CsRows8, centres: CsRows8, h: int, keep: int, work: Optional[int],
-                       stream: int) -> None:
-        self._check(self.lib.cs_rows8_coverage(ctypes.byref(a), ctypes.byref(centres), h, keep, work, stream), "cs_rows8_coverage")
-
     def fps_step_lanes(self, lanes, n_lanes: int, mode: int, stream: int) -> None:
         self._check(self.lib.cs_fps_step_lanes(lanes, n_lanes, mode, stream), "cs_fps_step_lanes")
 

@@ -18,44 +18,62 @@ int r8_grid(const int64_t groups, const DevInfo& d) {
     return (int)(groups < 1 ? 1 : (groups < cap ? groups : cap));
 }
 
-template <typename T, int G, int U = 1>
+// the widest load or store (16, 8, 4 or 2 bytes) that addresses, row stride and row length are whole multiples of
+int r8_width(const void* p, const int64_t stride_bytes, const int64_t row_bytes) {
+    const uintptr_t all = (uintptr_t)p | (uintptr_t)stride_bytes | (uintptr_t)row_bytes;
+    return (all & 15u) == 0 ? 16 : ((all & 7u) == 0 ? 8 : ((all & 3u) == 0 ? 4 : 2));
+}
+
+template <typename T, int G, int U, bool ROWS>
 int launch_rows8_write(const cs_rows8* r, const T* X, int64_t n, int64_t ld, int64_t start, cudaStream_t st, const DevInfo& d) {
-    const bool vec = ((uintptr_t)X & 15u) == 0 && (ld * sizeof(T)) % 16 == 0 && (r->dim & 7) == 0;
-    const int grid = r8_grid((n + kThreads / G - 1) / (kThreads / G), d);
-    if (vec) rows8_write_kernel<T, G, U, true><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
-    else rows8_write_kernel<T, G, U, false><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    constexpr int kMid = sizeof(T) == 4 ? 8 : 4, kOne = (int)sizeof(T);
+    const int width = r8_width(X, n > 1 ? ld * sizeof(T) : 0, (int64_t)r->dim * sizeof(T));
+    const int64_t rows = (int64_t)(kThreads / G) * (ROWS && width == 16 ? U : 1);
+    const int grid = r8_grid((n + rows - 1) / rows, d);
+    if (width == 16) rows8_write_kernel<T, G, U, ROWS, 16><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    else if (width >= kMid) rows8_write_kernel<T, G, 1, ROWS, kMid><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
+    else rows8_write_kernel<T, G, 1, ROWS, kOne><<<grid, kThreads, 0, st>>>(*r, X, n, ld, start);
     return check_launch();
 }
 template <typename T>
 int launch_rows8_write(const cs_rows8* r, const void* X, int64_t n, int64_t ld, int64_t start, cudaStream_t st, const DevInfo& d) {
     const T* x = static_cast<const T*>(X);
     if (((uintptr_t)X % sizeof(T)) != 0) return CS_E_ALIGN;
-    // the lanes that 8 elements each of the row (its first block) take: padding codes up to the pitch are theirs too
-    if (r->dim <= 16) return launch_rows8_write<T, 2>(r, x, n, ld, start, st, d);
-    if (r->dim <= 32) return launch_rows8_write<T, 4>(r, x, n, ld, start, st, d);
-    if (r->dim <= 64) return launch_rows8_write<T, 8>(r, x, n, ld, start, st, d);
-    if (r->dim <= 128) return launch_rows8_write<T, 16>(r, x, n, ld, start, st, d);
-    return launch_rows8_write<T, 16, 2>(r, x, n, ld, start, st, d);
+    // the lanes that 8 elements each of the row (its first block) take: padding codes up to the pitch are theirs too.
+    // 64 bytes in flight a lane where loads are 16 bytes wide (4M x 128 float32: 442 us, one row at a time 555); narrow loads are
+    // bound by their number and lose with fewer warps resident (2M x 50 float16: 116 us, four rows at a time 162)
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;
+    if (r->dim <= 16) return launch_rows8_write<T, 2, U, true>(r, x, n, ld, start, st, d);
+    if (r->dim <= 32) return launch_rows8_write<T, 4, U, true>(r, x, n, ld, start, st, d);
+    if (r->dim <= 64) return launch_rows8_write<T, 8, U, true>(r, x, n, ld, start, st, d);
+    if (r->dim <= 128) return launch_rows8_write<T, 16, U, true>(r, x, n, ld, start, st, d);
+    return launch_rows8_write<T, 16, U, false>(r, x, n, ld, start, st, d);
 }
 
-template <typename T, int G>
-int launch_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, T* out, int64_t ld, bool vec, cudaStream_t st, const DevInfo& d) {
-    const int grid = r8_grid((m + kThreads / G - 1) / (kThreads / G), d);
-    if (vec) rows8_read_kernel<T, G, true><<<grid, kThreads, 0, st>>>(*r, rows, m, out, ld);
-    else rows8_read_kernel<T, G, false><<<grid, kThreads, 0, st>>>(*r, rows, m, out, ld);
+template <typename T, int E, int G>
+int launch_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, T* out, int64_t ld, cudaStream_t st, const DevInfo& d) {
+    constexpr int R = 4;                            // 2M x 256 to float32: 452 us; R = 2: 532, R = 8: 472
+    const int64_t per_block = (int64_t)(kThreads / G) * R;
+    rows8_read_kernel<T, E, G, R><<<r8_grid((m + per_block - 1) / per_block, d), kThreads, 0, st>>>(*r, rows, m, out, ld);
     return check_launch();
+}
+template <typename T, int E>
+int launch_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, T* out, int64_t ld, cudaStream_t st, const DevInfo& d) {
+    const int chunks = r->dim / E;
+    if (chunks <= 4) return launch_rows8_read<T, E, 4>(r, rows, m, out, ld, st, d);
+    if (chunks <= 8) return launch_rows8_read<T, E, 8>(r, rows, m, out, ld, st, d);
+    if (chunks <= 16) return launch_rows8_read<T, E, 16>(r, rows, m, out, ld, st, d);
+    return launch_rows8_read<T, E, 32>(r, rows, m, out, ld, st, d);
 }
 template <typename T>
 int launch_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, void* out, int64_t ld, cudaStream_t st, const DevInfo& d) {
     T* o = static_cast<T*>(out);
     if (((uintptr_t)out % sizeof(T)) != 0) return CS_E_ALIGN;
-    constexpr int E = 16 / (int)sizeof(T);
-    const bool vec = ((uintptr_t)out & 15u) == 0 && (ld * sizeof(T)) % 16 == 0 && r->dim % E == 0;
-    const int chunks = vec ? r->dim / E : r->dim;
-    if (chunks <= 4) return launch_rows8_read<T, 4>(r, rows, m, o, ld, vec, st, d);
-    if (chunks <= 8) return launch_rows8_read<T, 8>(r, rows, m, o, ld, vec, st, d);
-    if (chunks <= 16) return launch_rows8_read<T, 16>(r, rows, m, o, ld, vec, st, d);
-    return launch_rows8_read<T, 32>(r, rows, m, o, ld, vec, st, d);
+    const int width = r8_width(out, m > 1 ? ld * sizeof(T) : 0, (int64_t)r->dim * sizeof(T));
+    if (width == 16) return launch_rows8_read<T, 16 / (int)sizeof(T)>(r, rows, m, o, ld, st, d);
+    if (width == 8) return launch_rows8_read<T, 8 / (int)sizeof(T)>(r, rows, m, o, ld, st, d);
+    if (width == 4 && sizeof(T) == 2) return launch_rows8_read<T, 2>(r, rows, m, o, ld, st, d);
+    return launch_rows8_read<T, 1>(r, rows, m, o, ld, st, d);
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

@@ -49,98 +49,145 @@ __device__ __forceinline__ float r8_widen(const float v) { return v; }
 __device__ __forceinline__ float r8_widen(const __half v) { return __half2float(v); }
 __device__ __forceinline__ float r8_widen(const __nv_bfloat16 v) { return __uint_as_float((unsigned)__bfloat16_as_ushort(v) << 16); }
 
-// 8 consecutive elements, 16-byte aligned
-__device__ __forceinline__ void r8_load8(const float* p, float (&x)[8]) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(p)), b = __ldcs(reinterpret_cast<const float4*>(p) + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-template <typename T>
-__device__ __forceinline__ void r8_load8(const T* p, float (&x)[8]) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
-    const unsigned w[4] = {a.x, a.y, a.z, a.w};
+// V bytes of memory as whole elements, widened (narrow loads share lines with the next ones: those are kept)
+template <typename T, int V>
+__device__ __forceinline__ void r8_load(const T* p, float* x) {
+    if constexpr (V == 16) {
+        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(p));
+        const unsigned w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const unsigned short lo = (unsigned short)(w[i] & 0xffffu), hi = (unsigned short)(w[i] >> 16);
-        x[2 * i] = r8_widen(*reinterpret_cast<const T*>(&lo));
-        x[2 * i + 1] = r8_widen(*reinterpret_cast<const T*>(&hi));
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                x[i] = __uint_as_float(w[i]);
+            } else {
+                const unsigned short lo = (unsigned short)(w[i] & 0xffffu), hi = (unsigned short)(w[i] >> 16);
+                x[2 * i] = r8_widen(*reinterpret_cast<const T*>(&lo));
+                x[2 * i + 1] = r8_widen(*reinterpret_cast<const T*>(&hi));
+            }
+        }
+    } else if constexpr (V == 8 && sizeof(T) == 4) {
+        const float2 a = __ldg(reinterpret_cast<const float2*>(p));
+        x[0] = a.x;
+        x[1] = a.y;
+    } else if constexpr (V == 4 && sizeof(T) == 2) {
+        const unsigned w = __ldg(reinterpret_cast<const unsigned*>(p));
+        const unsigned short lo = (unsigned short)(w & 0xffffu), hi = (unsigned short)(w >> 16);
+        x[0] = r8_widen(*reinterpret_cast<const T*>(&lo));
+        x[1] = r8_widen(*reinterpret_cast<const T*>(&hi));
+    } else {
+        static_assert(V == sizeof(T), "one element");
+        x[0] = r8_widen(__ldg(p));
     }
 }
+// 8 consecutive elements from element c of a row of D, zeros behind its end (D is whole loads)
+template <typename T, int V>
+__device__ __forceinline__ void r8_load8(const T* row, const int c, const int D, const bool live, float (&x)[8]) {
+    constexpr int E = V / (int)sizeof(T);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k += E)
+        if (live && c + k < D) r8_load<T, V>(row + c + k, x + k);
+}
 
-// G lanes own a row (8 consecutive elements a lane and block); G < 16 serves rows of one block and 8 G
-// elements at most.  U blocks are loaded before the first is worked on.  VEC: 16-byte loads (base and row stride 16-byte aligned, D a multiple of 8).
-template <typename T, int G, int U, bool VEC>
+// One block of a row in the registers of G lanes, 8 elements each: the codes of this lane, the exponent byte, this lane's part of the
+// squared norm.
+template <int G>
+__device__ __forceinline__ uint2 r8_quantise(float (&x)[8], unsigned& byte, float& part) {
+    unsigned top = 0u;                     // magnitudes of finite numbers order like their bits
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const unsigned m = __float_as_uint(x[k]) & 0x7fffffffu;
+        if (m >= 0x7f800000u) x[k] = __uint_as_float(0x7fc00000u);
+        else top = m > top ? m : top;
+    }
+#pragma unroll
+    for (int off = G / 2; off > 0; off >>= 1) {
+        const unsigned o = __shfl_xor_sync(kFull, top, off);
+        top = o > top ? o : top;
+    }
+    // amax = m * 2^E with 1 <= m < 2; 448 = 1.75 * 2^8
+    int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    e = e < kR8MinExp ? kR8MinExp : e;
+    const float inv = __uint_as_float((unsigned)(127 - e) << 23), scale = __uint_as_float((unsigned)(127 + e) << 23);
+    unsigned q[4];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        q[k] = to_e4m3x2(mul_keep(x[2 * k], inv), mul_keep(x[2 * k + 1], inv));
+        const float2 v = from_e4m3x2(q[k]);
+        sum = __fmaf_rn(v.x, v.x, sum);
+        sum = __fmaf_rn(v.y, v.y, sum);
+    }
+    byte = (unsigned)(e + 127);
+    part = __fmul_rn(__fmul_rn(sum, scale), scale);
+    return make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+}
+
+// Bound by HBM.  G lanes own a row, 8 consecutive elements a lane and block; G < 16 serves rows of 8 G elements at
+// most.  What a lane has in flight decides the rate, so U blocks are loaded before the first is worked on: of one row, or
+// (ROWS, rows of one block) of U rows.  V: bytes of a load.
+template <typename T, int G, int U, bool ROWS, int V>
 __global__ void __launch_bounds__(kThreads) rows8_write_kernel(const cs_rows8 r, const T* __restrict__ X, const int64_t n,
                                                                const int64_t ld, const int64_t start) {
     const int D = r.dim, blocks = (D + kR8Block - 1) / kR8Block, words = r8_words(D);
     const int64_t pitch = r8_pitch(D);
     const int lane = threadIdx.x & 31, sub = lane & (G - 1);
     const int64_t per_pass = (int64_t)gridDim.x * (kThreads / G);
-    // the whole warp takes the same number of passes: the shuffles below need all its lanes
-    for (int64_t first = (int64_t)blockIdx.x * (kThreads / G) + (threadIdx.x >> 5) * (32 / G); first < n; first += per_pass) {
-        const int64_t i = first + lane / G;
-        const bool live = i < n;
-        const T* src = X + (live ? i : 0) * ld;
-        const int64_t row = start + (live ? i : 0);
-        unsigned char* dst = reinterpret_cast<unsigned char*>(r.codes) + row * pitch;
-        float norm = 0.0f;
-        unsigned word = 0u;
-        for (int b0 = 0; b0 < blocks; b0 += U) {
-            float x[U][8];
+    unsigned char* codes = reinterpret_cast<unsigned char*>(r.codes);
+    unsigned char* scales = reinterpret_cast<unsigned char*>(r.scales);
+    // the whole warp takes the same number of passes: the shuffles need all its lanes
+    for (int64_t first = (int64_t)blockIdx.x * (kThreads / G) + (threadIdx.x >> 5) * (32 / G); first < n; first += per_pass * (ROWS ? U : 1)) {
+        float x[U][8], norm = 0.0f;
+        if (ROWS) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int c = (b0 + u) * kR8Block + 8 * sub;
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[u][k] = 0.0f;
-                if (VEC) {
-                    if (live && c < D) r8_load8(src + c, x[u]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        if (live && c + k < D) x[u][k] = r8_widen(src[c + k]);
-                }
+                const int64_t i = first + u * per_pass + lane / G;
+                r8_load8<T, V>(X + (i < n ? i : 0) * ld, 8 * sub, D, i < n, x[u]);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int b = b0 + u, c = b * kR8Block + 8 * sub;
-                if (U > 1 && b >= blocks) break;
-                unsigned top = 0u;         // magnitudes of finite numbers order like their bits
+                const int64_t i = first + u * per_pass + lane / G, row = start + i;
+                unsigned byte;
+                const uint2 q = r8_quantise<G>(x[u], byte, norm);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const unsigned m = __float_as_uint(x[u][k]) & 0x7fffffffu;
-                    if (m >= 0x7f800000u) x[u][k] = __uint_as_float(0x7fc00000u);
-                    else top = m > top ? m : top;
-                }
-#pragma unroll
-                for (int off = G / 2; off > 0; off >>= 1) {
-                    const unsigned o = __shfl_xor_sync(kFull, top, off);
-                    top = o > top ? o : top;
-                }
-                // amax = m * 2^E with 1 <= m < 2; 448 = 1.75 * 2^8
-                int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-                e = e < kR8MinExp ? kR8MinExp : e;
-                const float inv = __uint_as_float((unsigned)(127 - e) << 23), scale = __uint_as_float((unsigned)(127 + e) << 23);
-                unsigned q[4];
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    q[k] = to_e4m3x2(mul_keep(x[u][2 * k], inv), mul_keep(x[u][2 * k + 1], inv));
-                    const float2 v = from_e4m3x2(q[k]);
-                    sum = __fmaf_rn(v.x, v.x, sum);
-                    sum = __fmaf_rn(v.y, v.y, sum);
-                }
-                norm = __fadd_rn(norm, __fmul_rn(__fmul_rn(sum, scale), scale));
-                if (live && c < pitch) *reinterpret_cast<uint2*>(dst + c) = make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-                word |= (unsigned)(e + 127) << (8 * (b & 3));
-                if ((b & 3) == 3 || b == blocks - 1) {
-                    if (live && sub == 0)
-                        *reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(r.scales) + r8_scale_word(row, b >> 2, words)) = word;
-                    word = 0u;
+                for (int off = G / 2; off > 0; off >>= 1) norm = __fadd_rn(norm, __shfl_xor_sync(kFull, norm, off));
+                if (i < n) {
+                    if (8 * sub < pitch) *reinterpret_cast<uint2*>(codes + row * pitch + 8 * sub) = q;
+                    if (sub == 0) {
+                        *reinterpret_cast<unsigned*>(scales + r8_scale_word(row, 0, 1)) = byte;
+                        r.norms[row] = norm;
+                    }
                 }
             }
+        } else {
+            const int64_t i = first + lane / G, row = start + i;
+            const bool live = i < n;
+            const T* src = X + (live ? i : 0) * ld;
+            unsigned word = 0u;
+            for (int b0 = 0; b0 < blocks; b0 += U) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) r8_load8<T, V>(src, (b0 + u) * kR8Block + 8 * sub, D, live, x[u]);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int b = b0 + u, c = b * kR8Block + 8 * sub;
+                    if (b >= blocks) break;
+                    unsigned byte;
+                    float part;
+                    const uint2 q = r8_quantise<G>(x[u], byte, part);
+                    norm = __fadd_rn(norm, part);
+                    if (live && c < pitch) *reinterpret_cast<uint2*>(codes + row * pitch + c) = q;
+                    word |= byte << (8 * (b & 3));
+                    if ((b & 3) == 3 || b == blocks - 1) {
+                        if (live && sub == 0) *reinterpret_cast<unsigned*>(scales + r8_scale_word(row, b >> 2, words)) = word;
+                        word = 0u;
+                    }
+                }
+            }
+#pragma unroll
+            for (int off = G / 2; off > 0; off >>= 1) norm = __fadd_rn(norm, __shfl_xor_sync(kFull, norm, off));
+            if (live && sub == 0) r.norms[row] = norm;
         }
-#pragma unroll
-        for (int off = G / 2; off > 0; off >>= 1) norm = __fadd_rn(norm, __shfl_xor_sync(kFull, norm, off));
-        if (live && sub == 0) r.norms[row] = norm;
     }
 }
 
@@ -148,52 +195,58 @@ __device__ __forceinline__ void r8_narrow(float& o, const float v) { o = v; }
 __device__ __forceinline__ void r8_narrow(__half& o, const float v) { o = __float2half_rn(v); }
 __device__ __forceinline__ void r8_narrow(__nv_bfloat16& o, const float v) { o = __float2bfloat16_rn(v); }
 
-// G lanes own an output row.  VEC: a lane turns 16 / sizeof(T) codes into one 16-byte store.
-template <typename T, int G, bool VEC>
+// Bound by HBM.  G lanes own a row; E codes a lane make one store of up to 16 bytes; R rows are in flight.
+template <typename T, int E, int G, int R>
 __global__ void __launch_bounds__(kThreads) rows8_read_kernel(const cs_rows8 r, const int64_t* __restrict__ rows, const int64_t m,
                                                               T* __restrict__ out, const int64_t ld) {
-    constexpr int E = VEC ? 16 / (int)sizeof(T) : 1;
-    const int D = r.dim, words = r8_words(D);
-    const int64_t pitch = r8_pitch(D);
-    const int sub = threadIdx.x & (G - 1);
-    const float nan = __uint_as_float(0x7fc00000u);
-    for (int64_t i = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G; i < m; i += (int64_t)gridDim.x * (kThreads / G)) {
-        const int64_t row = rows ? __ldg(rows + i) : i;
-        const bool known = row >= 0 && row < r.count;
-        const unsigned char* src = reinterpret_cast<const unsigned char*>(r.codes) + (known ? row : 0) * pitch;
-        T* dst = out + i * ld;
+    const int D = r.dim, words = r8_words(D), sub = threadIdx.x & (G - 1);
+    const int64_t pitch = r8_pitch(D), groups = (int64_t)gridDim.x * (kThreads / G);
+    for (int64_t first = (int64_t)blockIdx.x * (kThreads / G) + threadIdx.x / G; first < m; first += groups * R) {
+        const unsigned char* src[R];
+        const unsigned char* sf[R];
+#pragma unroll
+        for (int u = 0; u < R; ++u) {
+            const int64_t i = first + u * groups, row = i < m ? (rows ? __ldg(rows + i) : i) : -1;
+            const bool known = row >= 0 && row < r.count;
+            src[u] = known ? reinterpret_cast<const unsigned char*>(r.codes) + row * pitch : nullptr;
+            sf[u] = reinterpret_cast<const unsigned char*>(r.scales) + (known ? r8_scale_word(row, 0, words) : 0);
+        }
         for (int c = sub * E; c < D; c += G * E) {
-            float v[E];
-            if (known) {
-                const int b = c / kR8Block;
-                const unsigned e = __ldg(reinterpret_cast<const unsigned char*>(r.scales) + r8_scale_word(row, b >> 2, words) + (b & 3));
-                const float scale = r8_scale_value(e);
-                if (E == 1) {
-                    v[0] = mul_keep(from_e4m3x2(__ldg(src + c)).x, scale);
-                } else {
-                    unsigned w[2];
-                    if (E == 8) {
-                        const uint2 a = __ldg(reinterpret_cast<const uint2*>(src + c));
-                        w[0] = a.x; w[1] = a.y;
-                    } else {
-                        w[0] = __ldg(reinterpret_cast<const unsigned*>(src + c)); w[1] = 0u;
-                    }
+            uint2 code[R];
+            unsigned exponent[R];
+            const int b = c / kR8Block, word = (b >> 2) * 512 + (b & 3);
 #pragma unroll
-                    for (int k = 0; k < E / 2; ++k) {
-                        const float2 p = from_e4m3x2((w[k >> 1] >> (16 * (k & 1))) & 0xffffu);
-                        v[(2 * k) % E] = mul_keep(p.x, scale);
-                        v[(2 * k + 1) % E] = mul_keep(p.y, scale);
-                    }
+            for (int u = 0; u < R; ++u) {
+                code[u] = make_uint2(0u, 0u);
+                exponent[u] = 255u;                                 // a row that is not there is NaN
+                if (src[u]) {
+                    if (E == 8) code[u] = __ldg(reinterpret_cast<const uint2*>(src[u] + c));
+                    else if (E == 4) code[u].x = __ldg(reinterpret_cast<const unsigned*>(src[u] + c));
+                    else if (E == 2) code[u].x = __ldg(reinterpret_cast<const unsigned short*>(src[u] + c));
+                    else code[u].x = __ldg(src[u] + c);
+                    exponent[u] = __ldg(sf[u] + word);
                 }
-            } else {
-#pragma unroll
-                for (int k = 0; k < E; ++k) v[k] = nan;
             }
-            __align__(16) T o[E];
 #pragma unroll
-            for (int k = 0; k < E; ++k) r8_narrow(o[k], v[k]);
-            if (VEC) __stcs(reinterpret_cast<uint4*>(dst + c), *reinterpret_cast<const uint4*>(o));
-            else dst[c] = o[0];
+            for (int u = 0; u < R; ++u) {
+                const int64_t i = first + u * groups;
+                if (i >= m) break;
+                const float scale = r8_scale_value(exponent[u]);
+                T* dst = out + i * ld + c;
+                const unsigned w[2] = {code[u].x, code[u].y};
+                __align__(16) T o[E < 2 ? 2 : E];
+#pragma unroll
+                for (int k = 0; k < E; k += 2) {
+                    const float2 v = from_e4m3x2(w[k >> 2] >> (8 * (k & 2)) & 0xffffu);
+                    r8_narrow(o[k], mul_keep(v.x, scale));
+                    r8_narrow(o[k + 1], mul_keep(v.y, scale));
+                }
+                constexpr int kBytes = E * (int)sizeof(T);
+                if (kBytes == 16) __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(o));
+                else if (kBytes == 8) __stcs(reinterpret_cast<uint2*>(dst), *reinterpret_cast<const uint2*>(o));
+                else if (E > 1) __stcs(reinterpret_cast<unsigned*>(dst), *reinterpret_cast<const unsigned*>(o));
+                else dst[0] = o[0];
+            }
         }
     }
 }
