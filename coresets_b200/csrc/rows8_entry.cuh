@@ -121,6 +121,38 @@ int r8_scale_map(CUtensorMap* map, void* base, const int dim, const int64_t coun
                : CS_E_ARG;
 }
 
+// Products leave by bulk stores of 32 lanes x `cols` where their rows follow the lanes and start on 16 bytes (bfloat16
+// 16384 x 8192 x 256: 70 us, by the readers' own stores 150), sets job.bulk_out.
+template <typename T>
+int r8_out_map(CUtensorMap* map, R8Job& job, const int cols) {
+    job.bulk_out = job.lane_stride == 1 && ((uintptr_t)job.out & 15u) == 0 && (job.col_stride * sizeof(T)) % 16 == 0 && job.col_stride >= job.n_lane;
+    if (!job.bulk_out) return CS_OK;
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return CS_E_DEVICE;
+    const cuuint64_t dims[2] = {(cuuint64_t)job.n_lane, (cuuint64_t)job.n_col}, strides[1] = {(cuuint64_t)job.col_stride * sizeof(T)};
+    const cuuint32_t box[2] = {32, (cuuint32_t)cols}, step[2] = {1, 1};
+    return encode(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, job.out, dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? CS_OK
+               : CS_E_ARG;
+}
+
+// Column tiles per work item, so that `workers` blocks (or pairs) with whole items each finish soonest: rounds x (tiles of an
+// item + what an item costs besides, about a quarter of a tile).  20 000 x 64 by 512: 79 lane tiles on 74 pairs are 2 rounds
+// of 3 tiles, or 4 rounds of 1.
+int r8_col_split(const int64_t lane_tiles, const int64_t col_tiles, const int64_t workers) {
+    int64_t best = col_tiles;
+    double least = 1e300;
+    for (int64_t want = 1; want <= col_tiles && want <= 2 * workers; ++want) {
+        const int64_t per = (col_tiles + want - 1) / want, items = lane_tiles * ((col_tiles + per - 1) / per);
+        const double cost = (double)((items + workers - 1) / workers) * ((double)per + 0.25);
+        if (cost < least * 0.999) { least = cost; best = per; }
+        if (items >= 64 * workers) break;                       // the last round is no longer worth more splits
+    }
+    return (int)best;
+}
+
 // what the pair kernel's extra step needs per column, rounded up to whole tiles: 16 bytes of digits, then scale words
 int64_t r8_norm_rows(const int64_t n_col) { return n_col <= 64 ? 0 : (n_col + kPairCols - 1) / kPairCols * kPairCols; }
 
@@ -147,22 +179,11 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
         if (!rc) rc = r8_map(&maps.norm, digits, 16, rows, 16, kPairCols / 2, false);
         if (!rc) rc = r8_scale_map(&maps.norm_sf, scales, 1, rows, 2);
         if (rc) return rc;
-        // few lane tiles: split the centres until every pair has work
-        int64_t want = (pairs + lane_tiles - 1) / lane_tiles;
-        want = want > job.col_tiles ? job.col_tiles : want;
-        job.col_split = (int)((job.col_tiles + want - 1) / want);
+        job.col_split = r8_col_split(lane_tiles, job.col_tiles, pairs);
     }
     if (!S::kNorms) {
-        // bulk stores where the products' rows start on 16 bytes (20 000 x 20 000 x 128 to float32: PERF us against 401)
-        job.bulk_out = job.lane_stride == 1 && ((uintptr_t)job.out & 15u) == 0 && (job.col_stride * sizeof(T)) % 16 == 0 && job.col_stride >= job.n_lane;
-        if (job.bulk_out) {
-            const cuuint64_t dims[2] = {(cuuint64_t)job.n_lane, (cuuint64_t)job.n_col}, strides[1] = {(cuuint64_t)job.col_stride * sizeof(T)};
-            const cuuint32_t box[2] = {32, kPairPart}, step[2] = {1, 1};
-            if (encode_tiled()(&maps.out, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, job.out, dims, strides, box,
-                               step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-                return CS_E_ARG;
-        }
+        rc = r8_out_map<T>(&maps.out, job, kPairPart);
+        if (rc) return rc;
     }
     static thread_local KernelTune tune;
     rc = tune_kernel(rows8_pair_kernel<WHAT, T>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
@@ -176,34 +197,18 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
 
 template <int NT, int WHAT, typename T>
 int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
-    CUtensorMap lane_map, col_map;
+    using S = R8Shape<NT, WHAT, T>;
+    CUtensorMap lane_map, col_map, out_map = {};
     int rc = r8_map(&lane_map, lanes->codes, lanes->dim, lanes->count, kR8Block, kR8Lanes, true);
-    if (rc) return rc;
-    rc = r8_map(&col_map, cols->codes, cols->dim, cols->count, kR8Block, NT, true);
+    if (!rc) rc = r8_map(&col_map, cols->codes, cols->dim, cols->count, kR8Block, NT, true);
+    if (!rc && WHAT == R8_PRODUCTS) rc = r8_out_map<T>(&out_map, job, NT);
     if (rc) return rc;
     static thread_local KernelTune tune;
-    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, R8Shape<NT>::kSmem, 192, nullptr);
+    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, S::kSmem, 192, nullptr);
     if (rc) return rc;
-    job.col_tiles = (int)((job.n_col + NT - 1) / NT);
-    const int64_t lane_tiles = (job.n_lane + kR8Lanes - 1) / kR8Lanes;
-    if (WHAT == R8_PRODUCTS) {
-        job.col_split = 1;
-    } else {
-        // few lane tiles: split the centres until every SM has work
-        int64_t want = (d.sms + lane_tiles - 1) / lane_tiles;
-        want = want > job.col_tiles ? job.col_tiles : want;
-        job.col_split = (int)((job.col_tiles + want - 1) / want);
-    }
-    job.splits = (job.col_tiles + job.col_split - 1) / job.col_split;
-    job.items = lane_tiles * job.splits;
-    if (WHAT == R8_COVERAGE && job.splits > 1 && !job.keep) {
-        rows8_fill_kernel<<<r8_grid((job.n_lane + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(
-            static_cast<float*>(job.out), job.n_lane, __builtin_huge_valf());
-        rc = check_launch();
-        if (rc) return rc;
-    }
+    job.items = (job.n_lane + kR8Lanes - 1) / kR8Lanes;
     const int grid = (int)(job.items < d.sms ? job.items : d.sms);
-    rows8_mma_kernel<NT, WHAT, T><<<grid, 192, R8Shape<NT>::kSmem, st>>>(lane_map, col_map, job);
+    rows8_mma_kernel<NT, WHAT, T><<<grid, 192, S::kSmem, st>>>(lane_map, col_map, out_map, job);
     return check_launch();
 }
 // the narrowest tile that holds all columns; pairs of SMs where 64 do not (coverage of 1M x 128 by 8192 centres:

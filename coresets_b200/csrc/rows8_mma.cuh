@@ -30,9 +30,9 @@ struct R8Job {
     const float* col_norms;
     int64_t n_lane, n_col;                          // rows of the two operands
     int D, words;
-    int col_tiles;                                  // tiles of NT columns
-    int col_split;                                  // column tiles of one work item
-    int splits;                                     // work items per lane tile
+    int col_tiles;                                  // column tiles, those of one work item, and work items per
+    int col_split;                                  // lane tile (rows8_pair.cuh; here one tile holds all columns)
+    int splits;
     int64_t items;                                  // lane tiles * splits
     void* out;                                      // products: P; coverage: h
     int64_t lane_stride, col_stride;                // products, in elements
@@ -49,6 +49,12 @@ __device__ __forceinline__ uint64_t umma_desc(const uint32_t smem, const uint32_
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, const int x, const int y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
+}
+// one bulk store, from shared memory, of a box of the map's; what of it lies past the last row or column is left out
+__device__ __forceinline__ void r8_store_tile(const CUtensorMap* map, const int x, const int y, const uint32_t smem) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(smem) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -115,19 +121,21 @@ __device__ __forceinline__ bool r8_wait_warp(uint64_t* b, const uint32_t parity,
     return __all_sync(kFull, r8_wait(b, parity, abort_flag));
 }
 
-template <int NT> struct R8Shape {
+template <int NT, int WHAT, typename T> struct R8Shape {
     static constexpr int kTileA = kR8Lanes * kR8Block, kTileB = NT * kR8Block;
     static constexpr int kStage = kTileA + kTileB + 1024;              // two tiles, two scale words of 128 rows
-    static constexpr int kStages = 8;
     static constexpr int kAcc = 256 / (NT < 32 ? 32 : NT);             // accumulators: 8, 8, 4; the way from a tile's last MMA to its
                                                                        // free accumulator is much longer than its few MMAs
-    static constexpr int kSmem = kStages * kStage + 1024;              // slack to align the tiles to 1 KB
+    static constexpr int kOut = WHAT == R8_PRODUCTS ? 4 * 32 * NT * (int)sizeof(T) : 0;     // the readers' products on their way out
+    static constexpr int kStages = kOut > 16384 ? 7 : 8;
+    static constexpr int kSmem = kStages * kStage + kOut + 1024;       // slack to align the tiles to 1 KB
 };
 
 template <int NT, int WHAT, typename T>
 __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant__ CUtensorMap lane_map,
-                                                           const __grid_constant__ CUtensorMap col_map, const R8Job job) {
-    using S = R8Shape<NT>;
+                                                           const __grid_constant__ CUtensorMap col_map,
+                                                           const __grid_constant__ CUtensorMap out_map, const R8Job job) {
+    using S = R8Shape<NT, WHAT, T>;
     constexpr int NC = NT < 32 ? NT : 32;                              // columns read back at a time
     extern __shared__ unsigned char s_raw[];
     __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_acc_full[S::kAcc], s_acc_empty[S::kAcc];
@@ -159,24 +167,19 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
         uint32_t n = 0;                                                // stages filled so far
         bool ok = true;
         for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
-            const int64_t lt = item / job.splits;
-            const int c0 = (int)(item % job.splits) * job.col_split;
-            const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
-            for (int ct = c0; ct < c1 && ok; ++ct)
-                for (int kb = 0; kb < kblocks; ++kb, ++n) {
-                    const uint32_t st = n % S::kStages, round = n / S::kStages;
-                    if (round > 0 && !r8_wait_warp(&s_empty[st], (round - 1) & 1u, s_abort)) { ok = false; break; }
-                    unsigned char* a = tiles + st * S::kStage;
-                    if (elect_one()) {
-                        mbar_expect_tx(&s_full[st], S::kStage);
-                        tma_tile(a, &lane_map, kb * kR8Block, (int)(lt * kR8Lanes), &s_full[st]);
-                        tma_tile(a + S::kTileA, &col_map, kb * kR8Block, ct * NT, &s_full[st]);
-                        bulk_load(a + S::kTileA + S::kTileB, job.lane_scales + (lt * job.words + (kb >> 2)) * 512, 512, &s_full[st]);
-                        bulk_load(a + S::kTileA + S::kTileB + 512, job.col_scales + ((int64_t)(ct * NT >> 7) * job.words + (kb >> 2)) * 512,
-                                  512, &s_full[st]);
-                    }
-                    __syncwarp();
+            for (int kb = 0; kb < kblocks; ++kb, ++n) {
+                const uint32_t st = n % S::kStages, round = n / S::kStages;
+                if (round > 0 && !r8_wait_warp(&s_empty[st], (round - 1) & 1u, s_abort)) { ok = false; break; }
+                unsigned char* a = tiles + st * S::kStage;
+                if (elect_one()) {
+                    mbar_expect_tx(&s_full[st], S::kStage);
+                    tma_tile(a, &lane_map, kb * kR8Block, (int)(item * kR8Lanes), &s_full[st]);
+                    tma_tile(a + S::kTileA, &col_map, kb * kR8Block, 0, &s_full[st]);
+                    bulk_load(a + S::kTileA + S::kTileB, job.lane_scales + (item * job.words + (kb >> 2)) * 512, 512, &s_full[st]);
+                    bulk_load(a + S::kTileA + S::kTileB + 512, job.col_scales + (kb >> 2) * 512, 512, &s_full[st]);
                 }
+                __syncwarp();
+            }
         }
         // no copy may be in flight when the block leaves: the last fills of every stage (already
         // complete unless a consumer gave up)
@@ -188,32 +191,29 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
         bool ok = true;
         // e4m3 x e4m3, K-major, float32 accumulators, exponent-only scales, M = 128
         constexpr uint32_t kIdesc = ((uint32_t)(NT >> 3) << 17) | (1u << 23) | ((uint32_t)(kR8Lanes >> 4) << 24);
-        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
-            const int c0 = (int)(item % job.splits) * job.col_split;
-            const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
-            for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
-                const uint32_t buf = t % S::kAcc, round = t / S::kAcc;
-                if (round > 0 && !r8_wait_warp(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
-                const uint32_t acc = tmem + buf * (256 / S::kAcc);
-                for (int kb = 0; kb < kblocks; ++kb, ++n) {
-                    const uint32_t st = n % S::kStages;
-                    if (!r8_wait_warp(&s_full[st], (n / S::kStages) & 1u, s_abort)) { ok = false; break; }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint32_t a = smem_u32(tiles + st * S::kStage), b = a + S::kTileA, sf = b + S::kTileB;
-                        const uint32_t sfa = tmem + kSf + st * 8, sfb = sfa + 4;
-                        tc_copy_scales(sfa, umma_desc(sf, 128, 0));
-                        tc_copy_scales(sfb, umma_desc(sf + 512, 128, 0));
-                        const uint32_t id = kIdesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
-                        const int left = job.D - kb * kR8Block, steps = left >= kR8Block ? 4 : (left + 31) >> 5;
-                        const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
-                        for (int k = 0; k < steps; ++k)
-                            tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, kb > 0 || k > 0);
-                        tc_commit(&s_empty[st]);
-                        if (kb == kblocks - 1) tc_commit(&s_acc_full[buf]);
-                    }
-                    __syncwarp();
+        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x, ++t) {
+            const uint32_t buf = t % S::kAcc, round = t / S::kAcc;
+            if (round > 0 && !r8_wait_warp(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * (256 / S::kAcc);
+            for (int kb = 0; kb < kblocks; ++kb, ++n) {
+                const uint32_t st = n % S::kStages;
+                if (!r8_wait_warp(&s_full[st], (n / S::kStages) & 1u, s_abort)) { ok = false; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t a = smem_u32(tiles + st * S::kStage), b = a + S::kTileA, sf = b + S::kTileB;
+                    const uint32_t sfa = tmem + kSf + st * 8, sfb = sfa + 4;
+                    tc_copy_scales(sfa, umma_desc(sf, 128, 0));
+                    tc_copy_scales(sfb, umma_desc(sf + 512, 128, 0));
+                    const uint32_t id = kIdesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+                    const int left = job.D - kb * kR8Block, steps = left >= kR8Block ? 4 : (left + 31) >> 5;
+                    const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
+                    for (int k = 0; k < steps; ++k)
+                        tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, kb > 0 || k > 0);
+                    tc_commit(&s_empty[st]);
+                    if (kb == kblocks - 1) tc_commit(&s_acc_full[buf]);
                 }
+                __syncwarp();
             }
         }
         // the tensor core may still read the stages of a drained block: wait for what was issued
@@ -225,59 +225,58 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         uint32_t t = 0;
         bool ok = true;
-        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
-            const int64_t lt = item / job.splits;
-            const int c0 = (int)(item % job.splits) * job.col_split;
-            const int c1 = c0 + job.col_split < job.col_tiles ? c0 + job.col_split : job.col_tiles;
-            const int64_t row = lt * kR8Lanes + quad * 32 + lane;
-            float best = __uint_as_float(0x7f800000u);
-            for (int ct = c0; ct < c1 && ok; ++ct, ++t) {
-                const uint32_t buf = t % S::kAcc;
-                if (WHAT == R8_COVERAGE) {
-                    // norms of the tile's centres; a column past the last centre can never be the nearest
-                    __syncwarp();
-                    for (int c = lane; c < NT; c += 32) {
-                        const int64_t col = (int64_t)ct * NT + c;
-                        s_norm[quad][c] = col < job.n_col ? __ldg(job.col_norms + col) : __uint_as_float(0x7f800000u);
-                    }
-                    __syncwarp();
-                }
-                ok = r8_wait_warp(&s_acc_full[buf], (t / S::kAcc) & 1u, s_abort);
-                if (!ok) break;
-                tc_fence_after();
-                for (int c = 0; c < NT; c += NC) {
-                    unsigned v[NC];
-                    tc_load(lanes + buf * (256 / S::kAcc) + c, v);
-                    if (WHAT == R8_PRODUCTS) {
-                        const int64_t col = (int64_t)ct * NT + c;
-                        T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride + col * job.col_stride;
-                        if (row < job.n_lane) {
+        if (WHAT == R8_COVERAGE) {
+            // the centres' norms; a column past the last centre can never be the nearest
+            for (int c = lane; c < NT; c += 32) s_norm[quad][c] = c < job.n_col ? __ldg(job.col_norms + c) : __uint_as_float(0x7f800000u);
+            __syncwarp();
+        }
+        for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x, ++t) {
+            const int64_t row = item * kR8Lanes + quad * 32 + lane;
+            const uint32_t buf = t % S::kAcc;
+            ok = r8_wait_warp(&s_acc_full[buf], (t / S::kAcc) & 1u, s_abort);
+            if (!ok) break;
+            tc_fence_after();
+            unsigned v[NT];
 #pragma unroll
-                            for (int j = 0; j < NC; ++j)
-                                if (col + j < job.n_col) {
-                                    T o;
-                                    r8_narrow(o, __uint_as_float(v[j]));
-                                    out[j * job.col_stride] = o;
-                                }
+            for (int c = 0; c < NT; c += NC) tc_load(lanes + buf * (256 / S::kAcc) + c, *reinterpret_cast<unsigned(*)[NC]>(v + c));
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_acc_empty[buf]);
+            if (WHAT == R8_PRODUCTS) {
+                if (job.bulk_out) {
+                    // NT columns x 32 lanes through shared memory, one bulk store for the warp
+                    T* mine = reinterpret_cast<T*>(tiles + S::kStages * S::kStage) + quad * (NT * 32);
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) r8_narrow(mine[j * 32 + lane], __uint_as_float(v[j]));
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && row < job.n_lane) r8_store_tile(&out_map, (int)row, 0, smem_u32(mine));
+                } else if (row < job.n_lane) {
+                    T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        if (j < job.n_col) {
+                            T o;
+                            r8_narrow(o, __uint_as_float(v[j]));
+                            out[j * job.col_stride] = o;
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < NC; ++j) best = fminf(best, __fmaf_rn(-2.0f, __uint_as_float(v[j]), s_norm[quad][c + j]));
-                    }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&s_acc_empty[buf]);
-            }
-            if (WHAT == R8_COVERAGE && ok && row < job.n_lane) {
+            } else if (row < job.n_lane) {
                 // |a - c|^2 = |a|^2 + (|c|^2 - 2 a.c); a NaN never lowers h, rounding never makes it negative
-                const float d = __fadd_rn(__ldg(job.lane_norms + row), best);
-                float* h = reinterpret_cast<float*>(job.out) + row;
+                float best[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) best[j] = __uint_as_float(0x7f800000u);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) best[j & 3] = fminf(best[j & 3], __fmaf_rn(-2.0f, __uint_as_float(v[j]), s_norm[quad][j]));
+                const float d = __fadd_rn(__ldg(job.lane_norms + row), fminf(fminf(best[0], best[1]), fminf(best[2], best[3])));
                 const float up = d == d ? fmaxf(d, 0.0f) : __uint_as_float(0x7f800000u);
-                if (job.splits > 1) atomicMin(reinterpret_cast<int*>(h), __float_as_int(up));   // up >= 0: ordered like its bits, and below it every negative h
-                else *h = job.keep ? fminf(*h, up) : up;
+                float* h = reinterpret_cast<float*>(job.out) + row;
+                *h = job.keep ? fminf(*h, up) : up;
             }
         }
+        if (WHAT == R8_PRODUCTS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     tc_fence_before();

@@ -293,11 +293,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                         for (int j = 0; j < kPairPart; ++j) r8_narrow(mine[j * 32 + lane], __uint_as_float(v[j]));
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0 && row < job.n_lane && col < job.n_col) {
-                            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
-                                         ::"l"(&maps.out), "r"((int)row), "r"((int)col), "r"(smem_u32(mine)) : "memory");
-                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                        }
+                        if (lane == 0 && row < job.n_lane && col < job.n_col) r8_store_tile(&maps.out, (int)row, (int)col, smem_u32(mine));
                     } else if (row < job.n_lane) {
                         T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride + col * job.col_stride;
 #pragma unroll
