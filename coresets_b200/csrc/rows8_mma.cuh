@@ -126,7 +126,8 @@ template <int NT, int WHAT, typename T> struct R8Shape {
     static constexpr int kStage = kTileA + kTileB + 1024;              // two tiles, two scale words of 128 rows
     static constexpr int kAcc = 256 / (NT < 32 ? 32 : NT);             // accumulators: 8, 8, 4; the way from a tile's last MMA to its
                                                                        // free accumulator is much longer than its few MMAs
-    static constexpr int kOut = WHAT == R8_PRODUCTS ? 4 * 32 * NT * (int)sizeof(T) : 0;     // the readers' products on their way out
+    static constexpr int kOutWarp = WHAT == R8_PRODUCTS ? (32 * (NT + 1) * (int)sizeof(T) + 127) & ~127 : 0;      // a reader's products on their way out
+    static constexpr int kOut = 4 * kOutWarp;
     static constexpr int kStages = kOut > 16384 ? 7 : 8;
     static constexpr int kSmem = kStages * kStage + kOut + 1024;       // slack to align the tiles to 1 KB
 };
@@ -243,16 +244,41 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_acc_empty[buf]);
             if (WHAT == R8_PRODUCTS) {
+                T* mine = reinterpret_cast<T*>(tiles + S::kStages * S::kStage + quad * S::kOutWarp);
                 if (job.bulk_out) {
                     // NT columns x 32 lanes through shared memory, one bulk store for the warp
-                    T* mine = reinterpret_cast<T*>(tiles + S::kStages * S::kStage) + quad * (NT * 32);
-                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < NT; ++j) r8_narrow(mine[j * 32 + lane], __uint_as_float(v[j]));
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0 && row < job.n_lane) r8_store_tile(&out_map, (int)row, 0, smem_u32(mine));
+                } else if (job.col_stride == 1) {
+                    // the rows of `out` follow the columns: 32 rows of n_col elements through shared memory, stored in
+                    // their order (1M x 64 x 128 to float32: 139 us, each lane storing its own row 360)
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) r8_narrow(mine[lane * (NT + 1) + j], __uint_as_float(v[j]));
+                    __syncwarp();
+                    const int n_col = (int)job.n_col, rows = (int)(job.n_lane - (row - lane) < 32 ? job.n_lane - (row - lane) : 32);
+                    const unsigned inverse = n_col > 1 ? (unsigned)((0x100000000ull + n_col - 1) / n_col) : 0u;
+                    T* out = reinterpret_cast<T*>(job.out) + (row - lane) * job.lane_stride;
+                    const int last = rows * n_col;
+#pragma unroll 1
+                    for (int e0 = lane; e0 < last; e0 += 8 * 32) {
+                        T o[8];
+                        int64_t at[8];
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) {
+                            const int e = e0 + 32 * u < last ? e0 + 32 * u : last - 1;      // (past the end: its last element again)
+                            const int r = n_col > 1 ? (int)__umulhi((unsigned)e, inverse) : e, c = e - r * n_col;
+                            o[u] = mine[r * (NT + 1) + c];
+                            at[u] = r * job.lane_stride + c;
+                        }
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) out[at[u]] = o[u];
+                    }
                 } else if (row < job.n_lane) {
                     T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride;
 #pragma unroll

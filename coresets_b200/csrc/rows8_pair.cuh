@@ -10,7 +10,7 @@
 // step of 32 elements: -|c|^2 / 2 is a 24-bit number, six digits of 4 bits that e4m3 holds exactly, times
 // six powers of two that stand in the lane operand, times one exponent per column.  The readers are left with one
 // three-input maximum per two columns.  Reading the norms from shared memory instead costs 4 wavefronts per
-// 16 bytes, and that pipe then sets the pace (1M x 128 by 8192 centres: 1.28 ms; with the extra step PERF).
+// 16 bytes, and that pipe then sets the pace (1M x 128 by 8192 centres: 1.28 ms; with the extra step 1.10 ms).
 //
 // The even block ("leader") issues every MMA; the full and the accumulator-free barriers are its own,
 // the stage-free and the accumulator-full barriers exist in both blocks and are reached by multicast commits.
