@@ -121,11 +121,13 @@ int r8_scale_map(CUtensorMap* map, void* base, const int dim, const int64_t coun
                : CS_E_ARG;
 }
 
-// Products leave by bulk stores of 32 lanes x `cols` where their rows follow the lanes and start on 16 bytes (bfloat16
-// 16384 x 8192 x 256: 70 us, by the readers' own stores 150), sets job.bulk_out.
+// Products leave by bulk stores of 32 lanes x `cols` where their rows follow the lanes and start and end on 16 bytes (a bulk
+// store is cut off at whole 16 bytes, not at elements); bfloat16 16384 x 8192 x 256: 70 us, by the readers' own stores 150.
+// Sets job.bulk_out.
 template <typename T>
 int r8_out_map(CUtensorMap* map, R8Job& job, const int cols) {
-    job.bulk_out = job.lane_stride == 1 && ((uintptr_t)job.out & 15u) == 0 && (job.col_stride * sizeof(T)) % 16 == 0 && job.col_stride >= job.n_lane;
+    job.bulk_out = job.lane_stride == 1 && ((uintptr_t)job.out & 15u) == 0 && (job.col_stride * sizeof(T)) % 16 == 0 &&
+                   (job.n_lane * sizeof(T)) % 16 == 0 && job.col_stride >= job.n_lane;
     if (!job.bulk_out) return CS_OK;
     EncodeTiled encode = encode_tiled();
     if (!encode) return CS_E_DEVICE;
@@ -298,6 +300,7 @@ int cs_rows8_products(const cs_rows8* a, const cs_rows8* b, void* out, int32_t d
     const cs_rows8* lanes = swap ? a : b;
     const cs_rows8* cols = swap ? b : a;
     R8Job job = r8_job(lanes, cols);
+    job.status = a->status;
     job.out = out;
     job.lane_stride = swap ? ld : 1;
     job.col_stride = swap ? 1 : ld;

@@ -21,7 +21,7 @@ namespace {
 
 enum { R8_PRODUCTS = 0, R8_COVERAGE = 1 };
 constexpr int kR8Lanes = 128;                       // rows of the lane operand in a tile
-constexpr unsigned long long kR8WaitNs = 2000000000ull;
+constexpr unsigned long long kR8WaitNs = 10000000000ull;      // the bound of every wait, that of the engine's pipes
 
 struct R8Job {
     const unsigned char* lane_scales;

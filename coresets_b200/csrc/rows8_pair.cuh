@@ -94,20 +94,20 @@ __device__ __forceinline__ void tc_load48(const uint32_t tmem, unsigned (&u)[48]
 }
 
 // Digits and exponents of -|c|^2 / 2 for the pair kernel, `rows` (whole tiles) of them, and h = +inf where asked.
-// |c|^2 = m 2^(E - 150) with 24 bits of m = sum_i d_i 16^i; the lane operand holds 2^-9, 2^-5, 2^-1, 2^3, 2^7, 2^7, so the
-// codes are -d_0 .. -d_4, -16 d_5 and the scale 2^(E - 142).  Below 2^-112 a norm counts as 0; NaN and infinity, and the
-// columns past the last, get the NaN scale: never the largest.
+// |c|^2 = m 2^(E - 150) with 24 bits of m = sum_i d_i 16^i; the lane operand holds 2^-9, 2^-5, 2^-1, 2^3, 2^7, 2^7 with the
+// scale 2^-15, so the codes are -d_0 .. -d_4, -16 d_5 and the scale 2^(E - 127): its byte is E.  Subnormal norms count as 0;
+// NaN and infinity, and the columns past the last, get the NaN scale: never the largest.
 __global__ void rows8_norm_digits_kernel(const float* __restrict__ norms, const int64_t n, const int64_t rows, unsigned char* digits,
                                          unsigned char* scales, float* h, const int64_t n_h) {
     const int64_t step = (int64_t)gridDim.x * blockDim.x, at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     for (int64_t i = at; i < rows; i += step) {
         const unsigned bits = i < n ? __float_as_uint(__fadd_rn(__ldg(norms + i), 0.0f)) : 0x7fc00000u;      // (+ 0: no negative zero)
-        const unsigned e = (bits >> 23) & 255u, m = e >= 15u ? (bits & 0x7fffffu) | 0x800000u : 0u;
+        const unsigned e = (bits >> 23) & 255u, m = e > 0u ? (bits & 0x7fffffu) | 0x800000u : 0u;
         uint4 q = make_uint4(0u, 0u, 0u, 0u);
         q.x = to_e4m3x2(-(float)(m & 15u), -(float)(m >> 4 & 15u)) | to_e4m3x2(-(float)(m >> 8 & 15u), -(float)(m >> 12 & 15u)) << 16;
         q.y = to_e4m3x2(-(float)(m >> 16 & 15u), -16.0f * (float)(m >> 20 & 15u));
         reinterpret_cast<uint4*>(digits)[i] = q;
-        *reinterpret_cast<unsigned*>(scales + r8_scale_word(i, 0, 1)) = (bits & 0x80000000u) || e == 255u ? 255u : (e >= 15u ? e - 15u : 0u);
+        *reinterpret_cast<unsigned*>(scales + r8_scale_word(i, 0, 1)) = (bits & 0x80000000u) ? 255u : e;
     }
     for (int64_t i = at; i < n_h; i += step) h[i] = __uint_as_float(0x7f800000u);
 }
@@ -149,7 +149,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
     if (S::kNorms) {
         // 128 equal rows of 32 codes without a swizzle: 16 bytes of a row, 8 rows a group; the second 16 are 0
         for (int i = threadIdx.x; i < (4096 + 512) / 4; i += blockDim.x)
-            reinterpret_cast<unsigned*>(s_power)[i] = i >= 1024 ? 0x7f7f7f7fu : (i < 512 && (i & 3) == 0 ? 0x50301001u : (i < 512 && (i & 3) == 1 ? 0x7070u : 0u));
+            reinterpret_cast<unsigned*>(s_power)[i] = i >= 1024 ? 0x70707070u : (i < 512 && (i & 3) == 0 ? 0x50301001u : (i < 512 && (i & 3) == 1 ? 0x7070u : 0u));
         if (threadIdx.x < kStages * 4)
             *reinterpret_cast<unsigned*>(tiles + kStages * S::kTile + (threadIdx.x >> 2) * S::kFirst + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

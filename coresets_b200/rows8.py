@@ -113,12 +113,16 @@ class RowStore:
         return self
 
     def _adopt(self, codes, scales, norms, dim, count):
-        self.codes, self.scales, self.norms = codes, scales, norms
+        self._codes, self._scales, self._norms = codes, scales, norms      # (read-only: the library holds their addresses)
         self.dim, self.capacity, self.device = dim, int(codes.shape[0]), codes.device
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = CsRows8(codes.data_ptr(), scales.data_ptr(), norms.data_ptr(), self._status.data_ptr(),
                           self.capacity, count, dim, 0)
         self._ref = ctypes.byref(self._c)
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    norms = property(lambda self: self._norms)
 
     @property
     def count(self) -> int:
@@ -145,7 +149,8 @@ class RowStore:
         return out
 
     def check_status(self) -> None:
-        """Synchronise and raise if a bounded wait inside a product over this store ran out."""
+        """Synchronise and raise if a bounded wait inside a ``row_products`` or ``coverage`` with this store as its first
+        argument ran out."""
         status = int(self._status.item())
         if status:
             raise RuntimeError(f"a bounded wait of a product over {self!r} ran out (status {status}); its result is not valid")

@@ -411,7 +411,8 @@ typedef struct cs_rows8 {
     void* codes;
     void* scales;
     float* norms;
-    int32_t* status;     /* device word, set to 4 when a bounded wait of a product ran out; may be NULL */
+    int32_t* status;     /* device word, set to 4 when a bounded wait of a product or coverage whose
+                            first store this is ran out (its result is not valid); may be NULL       */
     int64_t capacity;    /* rows that the arrays hold                                                */
     int64_t count;       /* rows in use: what reads and products take                                 */
     int32_t dim;

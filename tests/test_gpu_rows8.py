@@ -246,6 +246,68 @@ def test_products_out_and_nan():
     assert row_products(a, b.take([])).shape == (40, 0) and row_products(a.take([]), b).shape == (0, 21)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,k", [(5, 200), (60, 1000), (200, 5), (1000, 64), (1000, 33), (333, 200), (400, 1001), (129, 96)])
+def test_products_into_part_of_a_matrix(n, k, dtype):
+    """Rows of 16-byte multiples (bulk stores) and odd ones, at aligned and odd places: nothing beside the result is written."""
+    dim = 72
+    a, av = stored(n, dim, 30)
+    b, bv = stored(k, dim, 31)
+    want, off = product_bound(av, bv, dtype)
+    for pitch, first in ((-(-k // 8) * 8 + 16, 8), (k + 3, 1), (k, 0)):
+        wide = torch.full((n + 2, pitch), -1.0, dtype=dtype, device="cuda")
+        got = row_products(a, b, dtype=dtype, out=wide[1 : n + 1, first : first + k])
+        assert (np.abs(f64(got) - want) <= off).all()
+        wide[1 : n + 1, first : first + k] = -1.0
+        assert (wide == -1.0).all()
+
+
+def test_wide_rows():
+    dim = 20011
+    a, av = stored(70, dim, 32, 0.1)
+    b, bv = stored(90, dim, 33, 0.1)
+    want, off = product_bound(av, bv, torch.float32)
+    assert (np.abs(f64(row_products(a, b)) - want) <= off).all()
+    off = coverage_bound(av, bv, dim)
+    assert (np.abs(f64(coverage(a, b)) - ref.coverage(av, bv)) <= off).all()
+    assert torch.equal(read_rows(a).cpu(), torch.from_numpy(av).float())
+
+
+def test_offsets_past_32_bits():
+    """Codes past 4 GiB, and a result of more than 2^31 elements (bulk stores and the readers' own)."""
+    n, dim = 4_300_000, 1024
+    store = RowStore.from_tensors(torch.zeros(n, dim, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn),
+                                  torch.zeros(-(-n // 128), 2, 32, 4, 4, dtype=torch.uint8, device="cuda"), torch.zeros(n, device="cuda"), dim)
+    x = rows(300, dim, 40)
+    first = n - 301
+    quantise_rows(x.cuda(), store=store, start=first)
+    check_rows(store, first, x)
+    _, _, xv, _ = ref.quantise(f64(x))
+    assert not read_rows(store, torch.tensor([first - 1, n - 1], device="cuda")).any()
+    np.testing.assert_array_equal(f64(read_rows(store, torch.arange(first, n - 1, device="cuda"))), xv)
+    few, fv = stored(3, dim, 41)
+    want, off = product_bound(fv, xv, torch.float32)
+    got = row_products(few, store)
+    assert (np.abs(f64(got[:, first : n - 1]) - want) <= off).all() and not got[:, :first].any()
+    got = row_products(store, few)
+    assert (np.abs(f64(got[first : n - 1]) - want.T) <= off.T).all() and not got[:first].any()
+    part = store.take(torch.arange(first, first + 100, device="cuda"))
+    h = f64(coverage(store, part))
+    assert (np.abs(h[first : n - 1] - ref.coverage(xv, xv[:100])) <= coverage_bound(xv, xv[:100], dim)).all()
+    assert (np.abs(h[:first] - (xv[:100] ** 2).sum(1).min()) <= (xv[:100] ** 2).sum(1).min() * 1e-5).all()
+    del got, store, h
+    for k in (1_000_000, 1_000_001):
+        a, av = stored(2200, 16, 42)
+        x = rows(1000, 16, 43)
+        b = quantise_rows(x.cuda().repeat(-(-k // 1000), 1)[:k])
+        got = row_products(a, b, dtype=torch.bfloat16)
+        _, _, xv, _ = ref.quantise(f64(x))
+        want, off = product_bound(av, xv, torch.bfloat16)
+        for c in (0, k // 2000 * 1000, k // 1000 * 1000 - 1000):
+            assert (np.abs(f64(got[:, c : c + 1000]) - want) <= off).all()
+        del got
+
+
 # ---- coverage -------------------------------------------------------------------------------------------
 
 def coverage_bound(a, c, dim):
@@ -276,6 +338,26 @@ def test_coverage(n, k, dim):
     assert (np.abs(f64(h) - np.fmin(prior, want)) <= off).all()
     assert (f64(h)[prior == -1] == -1).all()
     a.check_status()
+
+
+@pytest.mark.parametrize("k", [20, 200])
+@pytest.mark.parametrize("scale", [2.0 ** -50, 2.0 ** -20, 2.0 ** 40, 2.0 ** 55])
+def test_coverage_of_small_and_large_numbers(k, scale):
+    dim = 100
+    a, av = stored(200, dim, 13, scale)
+    c, cv = stored(k, dim, 14, scale)
+    assert (np.abs(f64(coverage(a, c)) - ref.coverage(av, cv)) <= coverage_bound(av, cv, dim)).all()
+
+
+def test_coverage_of_the_same_rows_and_of_zeros():
+    x = rows(300, 90, 15)
+    x[7] = 0
+    a = quantise_rows(x.cuda())
+    _, _, av, _ = ref.quantise(f64(x))
+    h = f64(coverage(a, a))
+    assert (h <= coverage_bound(av, av, 90)).all() and h[7] == 0
+    zeros = quantise_rows(torch.zeros(100, 90, device="cuda"))
+    np.testing.assert_allclose(f64(coverage(a, zeros)), f64(a.norms), rtol=4 * U)
 
 
 def test_coverage_of_chosen_rows_and_parts():
@@ -343,6 +425,17 @@ def test_refusals():
         RowStore.from_tensors(a.codes, a.scales, a.norms, 32, count=5)
     with pytest.raises(ValueError, match="n_to_select"):
         coresets.fps_cuda(a, 3)
+
+
+def test_status_word_reaches_the_host():
+    a, b = quantise_rows(rows(4, 32).cuda()), quantise_rows(rows(4, 32).cuda())
+    row_products(a, b)
+    a.check_status()
+    a._status.fill_(4)                                            # what a kernel leaves whose bounded wait ran out
+    with pytest.raises(RuntimeError, match="ran out"):
+        a.check_status()
+    with pytest.raises(AttributeError):
+        a.codes = b.codes
 
 
 def test_from_tensors_shares_memory():
