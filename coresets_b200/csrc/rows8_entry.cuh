@@ -158,9 +158,9 @@ int r8_col_split(const int64_t lane_tiles, const int64_t col_tiles, const int64_
 // what the pair kernel's extra step needs per column, rounded up to whole tiles: 16 bytes of digits, then scale words
 int64_t r8_norm_rows(const int64_t n_col) { return n_col <= 64 ? 0 : (n_col + kPairCols - 1) / kPairCols * kPairCols; }
 
-template <int WHAT, typename T>
+template <int WHAT, typename T, bool KEEP>
 int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, void* work, cudaStream_t st, const DevInfo& d) {
-    using S = PairShape<WHAT, T>;
+    using S = PairShape<WHAT, T, KEEP>;
     PairMaps maps = {};
     int rc = r8_map(&maps.lane, lanes->codes, lanes->dim, lanes->count, kR8Block, kR8Lanes, true);
     if (!rc) rc = r8_map(&maps.col, cols->codes, cols->dim, cols->count, kR8Block, kPairCols / 2, true);
@@ -188,12 +188,12 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
         if (rc) return rc;
     }
     static thread_local KernelTune tune;
-    rc = tune_kernel(rows8_pair_kernel<WHAT, T>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
+    rc = tune_kernel(rows8_pair_kernel<WHAT, T, KEEP>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
     if (rc) return rc;
     job.splits = (job.col_tiles + job.col_split - 1) / job.col_split;
     job.items = lane_tiles * job.splits;
     const int grid = 2 * (int)(job.items < pairs ? job.items : pairs);
-    rows8_pair_kernel<WHAT, T><<<grid, kPairWarps * 32, S::kSmem, st>>>(maps, job);
+    rows8_pair_kernel<WHAT, T, KEEP><<<grid, kPairWarps * 32, S::kSmem, st>>>(maps, job);
     return check_launch();
 }
 
@@ -220,7 +220,8 @@ int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, vo
     if (job.n_col <= 16) return launch_rows8_mma<16, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 32) return launch_rows8_mma<32, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 64) return launch_rows8_mma<64, WHAT, T>(lanes, cols, job, st, d);
-    return launch_rows8_pair<WHAT, T>(lanes, cols, job, work, st, d);
+    if (WHAT == R8_COVERAGE && job.D <= kPairKept * kR8Block) return launch_rows8_pair<WHAT, T, WHAT == R8_COVERAGE>(lanes, cols, job, work, st, d);
+    return launch_rows8_pair<WHAT, T, false>(lanes, cols, job, work, st, d);
 }
 
 R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {

@@ -218,9 +218,10 @@ def quantise_rows(X: Tensor, *, store: Optional[RowStore] = None, start: Optiona
     return store
 
 
-def _result(out: Optional[Tensor], shape, dtype, device) -> Tensor:
+def _result(out: Optional[Tensor], shape, dtype, like: Tensor) -> Tensor:
+    device = like.device
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
         raise ValueError(f"out must be {dtype} of shape {tuple(shape)} on {device}, got {out.dtype} of shape {tuple(out.shape)} on {out.device}")
     if out.requires_grad:
@@ -240,7 +241,7 @@ def read_rows(store: RowStore, rows=None, *, dtype: torch.dtype = torch.float32,
     if rows is not None:
         rows = _row_numbers(store, rows)
     m = store.count if rows is None else rows.shape[0]
-    out = _result(out, (m, store.dim), dtype, store.device)
+    out = _result(out, (m, store.dim), dtype, store._norms)
     if m:
         _call(store.device, "cs_rows8_read", store._ref, None if rows is None else rows.data_ptr(), m, out.data_ptr(), code,
               out.stride(0) if m > 1 else store.dim)
@@ -262,7 +263,7 @@ def row_products(a: RowStore, b: RowStore, *, dtype: torch.dtype = torch.float32
     _check_pair(a, b, ("a", "b"))
     code = _dtype_code(dtype, "dtype")
     n, k = a.count, b.count
-    out = _result(out, (n, k), dtype, a.device)
+    out = _result(out, (n, k), dtype, a._norms)
     if n and k:
         _call(a.device, "cs_rows8_products", a._ref, b._ref, out.data_ptr(), code, out.stride(0) if n > 1 else k)
     return out
@@ -287,10 +288,10 @@ def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
         if h.requires_grad:
             raise ValueError("h must not require a gradient")
     else:
-        h = torch.empty(n, dtype=torch.float32, device=store.device)
+        h = store._norms.new_empty(n)
     if n:
         size = _native.get_native().lib.cs_rows8_coverage_bytes(centres.count)
-        work = torch.empty(size, dtype=torch.uint8, device=store.device) if size else None
+        work = store._norms.new_empty(size >> 2) if size else None
         _call(store.device, "cs_rows8_coverage", store._ref, centres._ref, h.data_ptr(), int(keep), work.data_ptr() if size else None)
     return h
 
