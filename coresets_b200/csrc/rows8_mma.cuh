@@ -182,6 +182,8 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
                 __syncwarp();
             }
         }
+        // the last releases of the stages have arrived before the block leaves
+        for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n && ok; ++k) ok = r8_wait_warp(&s_empty[k % S::kStages], (k / S::kStages) & 1u, s_abort);
         // no copy may be in flight when the block leaves: the last fills of every stage (already
         // complete unless a consumer gave up)
         if (!ok)

@@ -20,7 +20,7 @@
 namespace {
 
 constexpr int kPairCols = 192, kPairLanes = 256;
-constexpr int kPairReaders = 16, kPairWarps = 2 + kPairReaders;
+constexpr int kPairReaders = 16, kPairWarps = 3 + kPairReaders;
 constexpr int kPairPart = kPairCols / (kPairReaders / 4);        // columns of a reading warp
 constexpr int kPairA = kR8Lanes * kR8Block, kPairB = kPairCols / 2 * kR8Block;
 constexpr int kPairSf = 512 + 1024;                              // scale words of 128 lanes, and of the columns' two chunks of 128
@@ -37,8 +37,8 @@ template <int WHAT, typename T, bool KEEP> struct PairShape {
     static constexpr int kKept = KEEP ? kPairKept * kPairA : 0;                // lane operand of whole items
     static constexpr int kFirst = (kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0) + 127) & ~127;    // what else a stage may bring in (digits end with 16 zero bytes)
     static constexpr int kSmem = kKept + kStages * (kTile + kFirst) + kOut + 1024;
-    // TMEM columns of scales, one slot per 4 blocks of a row.  A slot comes round after kStages stages at
-    // least: the MMAs that read it are known to be done, since the stage itself was free to be filled again.
+    // TMEM columns of scales, one slot per 4 blocks of a row.  A slot comes round after kStages groups of at least one stage:
+    // the last stage of the group that had it was filled again, so its MMAs are done, before the group that gets it was.
     static constexpr int kSlot = kNorms ? 20 : 12;
 };
 static_assert(PairShape<R8_COVERAGE, float, true>::kSmem + 8192 <= 232448, "shared memory");
@@ -148,10 +148,17 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
     const int64_t first = blockIdx.x >> 1, stride = gridDim.x >> 1;
     const int kblocks = (job.D + kR8Block - 1) / kR8Block;
     const uint32_t kept_slots = 2 * kblocks <= kPairKept ? 2 : 1;
+    // Two warps issue, one for each accumulator, tile by tile in turn: the way of one warp through a tile (waits, scales, MMAs,
+    // commits) is longer than the MMAs of a narrow tile take (D = 128: 860 clocks for 480).  Only where two tiles fit the
+    // ring of stages.  A wait names the parity of a stage's fill, so it must not begin before the fill kStages earlier has
+    // completed.  A warp that begins tile t + 1 has seen its accumulator free, so the readers are through tile t - 1 and every
+    // fill up to that tile's last stage is complete; the stages of t + 1 end 2 kblocks later, and 2 kblocks <= kStages keeps
+    // the fills kStages earlier among those.  Wider rows, whose MMAs take longer than their issue, have one issuing warp.
+    const bool two = 2 * kblocks <= kStages;
     if (threadIdx.x == 0) {
         s_abort_word = 0;
         for (int i = 0; i < kStages; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 2 * kPairReaders); mbar_init(&s_kept_full[i], 1); mbar_init(&s_kept_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 2 * kPairReaders); mbar_init(&s_kept_full[i], 1); mbar_init(&s_kept_empty[i], two ? 2 : 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (S::kNorms) {
@@ -213,6 +220,8 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     if (++st == kStages) { st = 0; phase ^= 1u; }
                 }
         }
+        // the last releases of the stages reach both blocks: neither leaves before they have
+        for (uint32_t k = n > kStages ? n - kStages : 0; k < n && ok; ++k) ok = r8_wait_warp(&s_empty[k % kStages], (k / kStages) & 1u, s_abort);
         // no copy may be in flight when the pair leaves (they all are complete unless a role gave up)
         if (!ok && rank == 0) {
             for (uint32_t k = n > kStages ? n - kStages : 0; k < n; ++k)
@@ -220,15 +229,14 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             for (uint32_t k = items > kept_slots ? items - kept_slots : 0; k < items; ++k)
                 for (int it = 0; it < (1 << 16) && !mbar_try(&s_kept_full[k % kept_slots], (k / kept_slots) & 1u); ++it) {}
         }
-    } else if (warp == 1) {
-        if (rank == 0) {
-            uint32_t st = 0, phase = 0, slot = 0;
-            uint32_t n = 0, t = 0, items = 0;
-            bool ok = true;
+    } else if (warp <= 2) {
+        const uint32_t own = (uint32_t)warp - 1;
+        if (rank == 0 && (two || own == 0)) {
+            const uint32_t groups = (uint32_t)(kblocks + 3) >> 2;
+            uint32_t n = 0, t = 0, items = 0;                       // stages, tiles and items so far, the other warp's among them
+            bool ok = true, fresh = true;
             constexpr uint32_t kIdesc = ((uint32_t)(kPairCols >> 3) << 17) | (1u << 23) | ((uint32_t)(kPairLanes >> 4) << 24);
             const uint32_t base = smem_u32(tiles), power = smem_u32(s_power), sf_power = tmem + kSf + kStages * S::kSlot;
-            if (S::kNorms && elect_one()) pair_copy_scales(sf_power, umma_desc(power + 4096, 128, 0));
-            __syncwarp();
             for (int64_t item = first; item < job.items && ok; item += stride) {
                 const PairSpan sp = pair_span(job, item);
                 const uint32_t kept_slot = items % kept_slots, kept_at = smem_u32(kept) + kept_slot * (kPairKept / 2) * kPairA;
@@ -236,18 +244,25 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                 ++items;
                 for (int ct = sp.c0; ct < sp.c1 && ok; ++ct, ++t) {
                     const uint32_t buf = t & 1u, round = t >> 1;
+                    if (two && buf != own) {
+                        n += (uint32_t)kblocks;
+                        continue;
+                    }
                     if (round > 0 && !r8_wait_warp(&s_acc_empty[buf], (round - 1) & 1u, s_abort)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t acc = tmem + buf * kPairCols;
                     // the tile's first column within its chunk of 128 scales: 32 rows a TMEM column
                     const uint32_t sub = (uint32_t)(ct * kPairCols & 127) >> 5;
+                    uint32_t slot = t * groups % kStages, st = n % kStages, phase = n / kStages & 1u;
                     for (int kb = 0; kb < kblocks; ++kb, ++n) {
                         if (!r8_wait_warp(&s_full[st], phase, s_abort)) { ok = false; break; }
                         tc_fence_after();
-                        if ((kb & 3) == 0 && ++slot == kStages) slot = 0;
+                        if (kb > 0 && (kb & 3) == 0 && ++slot == kStages) slot = 0;
                         if (elect_one()) {
                             const uint32_t b = base + (st + 1) * S::kTile - kPairB, a = KEEP ? kept_at + kb * kPairA : b - kPairA, sf = base + kStages * S::kTile + st * S::kFirst, norm = sf + kPairSf;
                             const uint32_t sfa = tmem + kSf + slot * S::kSlot, sfb = sfa + 4;
+                            // (the lane operand's powers for the norms: by each warp before its own MMAs)
+                            if (S::kNorms && fresh) pair_copy_scales(sf_power, umma_desc(power + 4096, 128, 0));
                             if ((kb & 3) == 0) {
                                 pair_copy_scales(sfa, umma_desc(sf, 128, 0));
                                 pair_copy_scales(sfb, umma_desc(sf + 512, 128, 0));
@@ -272,22 +287,24 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                                          sfb + 8 + sub, true);
                             }
                             pair_commit(&s_empty[st]);
-                            if (kb == kblocks - 1) {
-                                pair_commit(&s_acc_full[buf]);
-                                if (KEEP && ct == sp.c1 - 1) pair_commit(&s_kept_empty[kept_slot]);
-                            }
+                            if (kb == kblocks - 1) pair_commit(&s_acc_full[buf]);
                         }
                         __syncwarp();
+                        fresh = false;
                         if (++st == kStages) { st = 0; phase ^= 1u; }
                     }
                 }
+                // (only where the slot is filled again: nobody would wait for the last of these)
+                if (KEEP && ok && item + stride * kept_slots < job.items && elect_one()) pair_commit(&s_kept_empty[kept_slot]);
+                __syncwarp();
             }
+            // the tensor cores may still read the stages of a drained pair: wait for what was issued
             if (!ok)
                 for (uint32_t k = n > kStages ? n - kStages : 0; k < n; ++k)
                     for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % kStages], (k / kStages) & 1u); ++it) {}
         }
     } else {
-        const int quad = warp & 3, part = (warp - 2) >> 2;
+        const int quad = warp & 3, part = (warp - 3) >> 2;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + part * kPairPart;
         const float low = __uint_as_float(0xff800000u);
         uint32_t t = 0;
@@ -314,7 +331,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     if (job.bulk_out) {
                         // 48 columns x 32 lanes through shared memory, one bulk store for the warp (it leaves out what lies
                         // past the last lane or column)
-                        T* mine = reinterpret_cast<T*>(tiles + kStages * (S::kTile + S::kFirst)) + (warp - 2) * (kPairPart * 32);
+                        T* mine = reinterpret_cast<T*>(tiles + kStages * (S::kTile + S::kFirst)) + (warp - 3) * (kPairPart * 32);
                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
 #pragma unroll
