@@ -140,21 +140,6 @@ int r8_out_map(CUtensorMap* map, R8Job& job, const int cols) {
                : CS_E_ARG;
 }
 
-// Column tiles per work item, so that `workers` blocks (or pairs) with whole items each finish soonest: rounds x (tiles of an
-// item + what an item costs besides, about a quarter of a tile).  20 000 x 64 by 512: 79 lane tiles on 74 pairs are 2 rounds
-// of 3 tiles, or 4 rounds of 1.
-int r8_col_split(const int64_t lane_tiles, const int64_t col_tiles, const int64_t workers) {
-    int64_t best = col_tiles;
-    double least = 1e300;
-    for (int64_t want = 1; want <= col_tiles && want <= 2 * workers; ++want) {
-        const int64_t per = (col_tiles + want - 1) / want, items = lane_tiles * ((col_tiles + per - 1) / per);
-        const double cost = (double)((items + workers - 1) / workers) * ((double)per + 0.25);
-        if (cost < least * 0.999) { least = cost; best = per; }
-        if (items >= 64 * workers) break;                       // the last round is no longer worth more splits
-    }
-    return (int)best;
-}
-
 // what the pair kernel's extra step needs per column, rounded up to whole tiles: 16 bytes of digits, then scale words
 int64_t r8_norm_rows(const int64_t n_col) { return n_col <= 64 ? 0 : (n_col + kPairCols - 1) / kPairCols * kPairCols; }
 
@@ -169,7 +154,7 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
     if (rc) return rc;
     const int64_t pairs = d.sms / 2, lane_tiles = (job.n_lane + kPairLanes - 1) / kPairLanes;
     job.col_tiles = (int)((job.n_col + kPairCols - 1) / kPairCols);
-    job.col_split = 1;
+    job.tiles = lane_tiles * job.col_tiles;
     if (S::kNorms) {
         const int64_t rows = r8_norm_rows(job.n_col);
         unsigned char* digits = static_cast<unsigned char*>(work);
@@ -181,7 +166,6 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
         if (!rc) rc = r8_map(&maps.norm, digits, 16, rows, 16, kPairCols / 2, false);
         if (!rc) rc = r8_scale_map(&maps.norm_sf, scales, 1, rows, 2);
         if (rc) return rc;
-        job.col_split = r8_col_split(lane_tiles, job.col_tiles, pairs);
     }
     if (!S::kNorms) {
         rc = r8_out_map<T>(&maps.out, job, kPairPart);
@@ -190,9 +174,7 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
     static thread_local KernelTune tune;
     rc = tune_kernel(rows8_pair_kernel<WHAT, T, KEEP>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
     if (rc) return rc;
-    job.splits = (job.col_tiles + job.col_split - 1) / job.col_split;
-    job.items = lane_tiles * job.splits;
-    const int grid = 2 * (int)(job.items < pairs ? job.items : pairs);
+    const int grid = 2 * (int)(job.tiles < pairs ? job.tiles : pairs);
     rows8_pair_kernel<WHAT, T, KEEP><<<grid, kPairWarps * 32, S::kSmem, st>>>(maps, job);
     return check_launch();
 }
@@ -220,7 +202,8 @@ int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, vo
     if (job.n_col <= 16) return launch_rows8_mma<16, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 32) return launch_rows8_mma<32, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 64) return launch_rows8_mma<64, WHAT, T>(lanes, cols, job, st, d);
-    if (WHAT == R8_COVERAGE && job.D <= kPairKept * kR8Block) return launch_rows8_pair<WHAT, T, WHAT == R8_COVERAGE>(lanes, cols, job, work, st, d);
+    constexpr bool kMayKeep = WHAT == R8_COVERAGE;
+    if (kMayKeep && job.D <= kPairKept * kR8Block) return launch_rows8_pair<WHAT, T, kMayKeep>(lanes, cols, job, work, st, d);
     return launch_rows8_pair<WHAT, T, false>(lanes, cols, job, work, st, d);
 }
 

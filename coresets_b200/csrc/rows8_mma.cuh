@@ -30,10 +30,9 @@ struct R8Job {
     const float* col_norms;
     int64_t n_lane, n_col;                          // rows of the two operands
     int D, words;
-    int col_tiles;                                  // column tiles, those of one work item, and work items per
-    int col_split;                                  // lane tile (rows8_pair.cuh; here one tile holds all columns)
-    int splits;
-    int64_t items;                                  // lane tiles * splits
+    int col_tiles;                                  // rows8_pair.cuh: column tiles, and tiles in all
+    int64_t tiles;
+    int64_t items;                                  // here: lane tiles (one tile holds all columns)
     void* out;                                      // products: P; coverage: h
     int64_t lane_stride, col_stride;                // products, in elements
     int bulk_out;                                   // products: out takes bulk stores

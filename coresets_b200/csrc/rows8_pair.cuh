@@ -25,8 +25,8 @@ constexpr int kPairPart = kPairCols / (kPairReaders / 4);        // columns of a
 constexpr int kPairA = kR8Lanes * kR8Block, kPairB = kPairCols / 2 * kR8Block;
 constexpr int kPairSf = 512 + 1024;                              // scale words of 128 lanes, and of the columns' two chunks of 128
 constexpr int kPairNormB = kPairCols / 2 * 16, kPairNormSf = 1024;          // digits of the norms, and their exponents
-// KEEP: the lane operand of an item (128 rows of at most 8 blocks, two items where they have at most 4) stays in shared
-// memory while the item's column tiles pass, instead of coming in with every stage.  The MMAs take as many clocks as before,
+// KEEP: the lane operand of a segment (128 rows of at most 8 blocks, two segments where they have at most 4) stays in shared
+// memory while its column tiles pass, instead of coming in with every stage.  The MMAs take as many clocks as before,
 // but the SMs draw less power and clock higher: 500k x 256 by 10 000 centres 1073 -> 1024 us, 300k x 1024 by 8192 1720 -> 1615.
 constexpr int kPairKept = 8;
 template <int WHAT, typename T, bool KEEP> struct PairShape {
@@ -34,14 +34,15 @@ template <int WHAT, typename T, bool KEEP> struct PairShape {
     static constexpr int kOut = kNorms ? 0 : kPairReaders * kPairPart * 32 * (int)sizeof(T);     // a reading warp's share of a tile of products
     static constexpr int kStages = KEEP ? 5 : (!kNorms && sizeof(T) == 4 ? 4 : 6);
     static constexpr int kTile = (KEEP ? 0 : kPairA) + kPairB;                 // codes of a stage
-    static constexpr int kKept = KEEP ? kPairKept * kPairA : 0;                // lane operand of whole items
+    static constexpr int kKept = KEEP ? kPairKept * kPairA : 0;                // lane operand of whole segments
     static constexpr int kFirst = (kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0) + 127) & ~127;    // what else a stage may bring in (digits end with 16 zero bytes)
     static constexpr int kSmem = kKept + kStages * (kTile + kFirst) + kOut + 1024;
     // TMEM columns of scales, one slot per 4 blocks of a row.  A slot comes round after kStages groups of at least one stage:
     // the last stage of the group that had it was filled again, so its MMAs are done, before the group that gets it was.
     static constexpr int kSlot = kNorms ? 20 : 12;
 };
-static_assert(PairShape<R8_COVERAGE, float, true>::kSmem + 8192 <= 232448, "shared memory");
+static_assert(PairShape<R8_COVERAGE, float, true>::kSmem + 8192 <= 232448 && PairShape<R8_PRODUCTS, __half, false>::kSmem + 512 <= 232448 &&
+              PairShape<R8_PRODUCTS, float, false>::kSmem + 512 <= 232448, "shared memory");
 static_assert(2 * kPairCols + 6 * 20 + 4 <= 512 && 2 * kPairCols + 6 * 12 <= 512, "TMEM columns");
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -118,12 +119,21 @@ __global__ void rows8_norm_digits_kernel(const float* __restrict__ norms, const 
     for (int64_t i = at; i < n_h; i += step) h[i] = __uint_as_float(0x7f800000u);
 }
 
-struct PairSpan { int64_t lt; int c0, c1; };
-__device__ __forceinline__ PairSpan pair_span(const R8Job& job, const int64_t item) {
+// Which tiles a pair works on, as segments [c0, c1) of column tiles of one lane tile.  All tiles stand in one sequence, lane
+// tile by lane tile.  RUNS (coverage): the sequence is cut into equal runs, one per pair, so that a lane tile stays as long as
+// it can.  Otherwise (products) tile by tile in turn: pairs that run at the same time share operands in L2 and write
+// neighbouring parts of the result's rows (8192^3 to bfloat16: 408 us, in runs 511; 4096 x 100 000 x 128: 197, in runs 243).
+struct PairSpan {
+    int64_t lt, next;
+    int c0, c1;
+};
+template <bool RUNS>
+__device__ __forceinline__ PairSpan pair_span(const R8Job& job, const int64_t at, const int64_t last) {
     PairSpan s;
-    s.lt = item / job.splits;
-    s.c0 = (int)(item % job.splits) * job.col_split;
-    s.c1 = s.c0 + job.col_split < job.col_tiles ? s.c0 + job.col_split : job.col_tiles;
+    s.lt = at / job.col_tiles;
+    s.c0 = (int)(at - s.lt * job.col_tiles);
+    s.c1 = !RUNS ? s.c0 + 1 : (last - at < job.col_tiles - s.c0 ? s.c0 + (int)(last - at) : job.col_tiles);
+    s.next = RUNS ? at + (s.c1 - s.c0) : at + (gridDim.x >> 1);
     return s;
 }
 
@@ -145,7 +155,8 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
 
     const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;    // warp: known to be uniform
     const uint32_t rank = cluster_rank();
-    const int64_t first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+    const int64_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const int64_t first = S::kNorms ? job.tiles * pair / pairs : pair, last = S::kNorms ? job.tiles * (pair + 1) / pairs : job.tiles;
     const int kblocks = (job.D + kR8Block - 1) / kR8Block;
     const uint32_t kept_slots = 2 * kblocks <= kPairKept ? 2 : 1;
     // Two warps issue, one for each accumulator, tile by tile in turn: the way of one warp through a tile (waits, scales, MMAs,
@@ -184,8 +195,9 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
         uint32_t st = 0, phase = 0;
         uint32_t n = 0, items = 0;
         bool ok = true;
-        for (int64_t item = first; item < job.items && ok; item += stride) {
-            const PairSpan sp = pair_span(job, item);
+        for (int64_t at = first; at < last && ok;) {
+            const PairSpan sp = pair_span<S::kNorms>(job, at, last);
+            at = sp.next;
             const int row = (int)(sp.lt * kPairLanes) + (int)rank * kR8Lanes;
             if (KEEP) {
                 const uint32_t slot = items % kept_slots, round = items / kept_slots;
@@ -237,8 +249,9 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             bool ok = true, fresh = true;
             constexpr uint32_t kIdesc = ((uint32_t)(kPairCols >> 3) << 17) | (1u << 23) | ((uint32_t)(kPairLanes >> 4) << 24);
             const uint32_t base = smem_u32(tiles), power = smem_u32(s_power), sf_power = tmem + kSf + kStages * S::kSlot;
-            for (int64_t item = first; item < job.items && ok; item += stride) {
-                const PairSpan sp = pair_span(job, item);
+            for (int64_t at = first; at < last && ok;) {
+                const PairSpan sp = pair_span<S::kNorms>(job, at, last);
+                at = sp.next;
                 const uint32_t kept_slot = items % kept_slots, kept_at = smem_u32(kept) + kept_slot * (kPairKept / 2) * kPairA;
                 if (KEEP && !r8_wait_warp(&s_kept_full[kept_slot], items / kept_slots & 1u, s_abort)) { ok = false; break; }
                 ++items;
@@ -295,7 +308,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     }
                 }
                 // (only where the slot is filled again: nobody would wait for the last of these)
-                if (KEEP && ok && item + stride * kept_slots < job.items && elect_one()) pair_commit(&s_kept_empty[kept_slot]);
+                if (KEEP && ok && (last - 1) / job.col_tiles - sp.lt >= kept_slots && elect_one()) pair_commit(&s_kept_empty[kept_slot]);
                 __syncwarp();
             }
             // the tensor cores may still read the stages of a drained pair: wait for what was issued
@@ -309,8 +322,9 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
         const float low = __uint_as_float(0xff800000u);
         uint32_t t = 0;
         bool ok = true;
-        for (int64_t item = first; item < job.items && ok; item += stride) {
-            const PairSpan sp = pair_span(job, item);
+        for (int64_t at = first; at < last && ok;) {
+            const PairSpan sp = pair_span<S::kNorms>(job, at, last);
+            at = sp.next;
             const int64_t row = sp.lt * kPairLanes + rank * kR8Lanes + quad * 32 + lane;
             float best[4] = {low, low, low, low};
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct, ++t) {
