@@ -4,6 +4,8 @@
                                                                          (no CUDA graphs): cell-index kernels
     python -m coresets_b200.profile_cases dense <workload> <rows>       six dense picks: the bulk-copy kernel
     python -m coresets_b200.profile_cases dense16 <workload> <rows>     the same over float16 rows
+    python -m coresets_b200.profile_cases rows8 <workload> <rows> <k>   the rows in 8 bits: written, read back as float16, the
+                                                                         first k as centres of all, products with the first 8192
 
 Rows are the first <rows> of the named synthetic workload (coresets_b200/synth.py), generated on
 the device.
@@ -24,7 +26,7 @@ def main(argv) -> None:
     from .synth import WORKLOADS, MixtureSource, scaled
     dev = torch.device("cuda", 0)
     torch.cuda.set_device(0)
-    k = int(argv[3]) if what == "cells" else 16
+    k = int(argv[3]) if what in ("cells", "rows8") else 16
     X = MixtureSource(scaled(WORKLOADS[wname], rows, k=k)).rows(0, rows, dev)
     if what == "cells":
         sel = fps_cuda(X, k)
@@ -42,6 +44,17 @@ def main(argv) -> None:
             eng.step()
         eng.check_status()
         print("done", wname, rows)
+    elif what == "rows8":
+        from . import coverage, quantise_rows, read_rows, row_products
+        store = quantise_rows(X)
+        centres, some = store.take(torch.arange(k)), store.take(torch.arange(min(rows, 8192)))
+        for _ in range(3):
+            quantise_rows(X, store=store, start=0)
+            read_rows(store, dtype=torch.float16)
+            h = coverage(store, centres)
+            row_products(some, centres, dtype=torch.bfloat16)
+        store.check_status()
+        print("done", wname, rows, k, float(h.max()))
     else:
         raise SystemExit(__doc__)
 
