@@ -39,11 +39,12 @@ __device__ __forceinline__ unsigned to_e4m3x2(const float lo, const float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ float2 from_e4m3x2(const unsigned codes) {
+__device__ __forceinline__ __half2 half_from_e4m3x2(const unsigned codes) {
     unsigned h2;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((unsigned short)codes));
-    return __half22float2(*reinterpret_cast<const __half2*>(&h2));
+    return *reinterpret_cast<const __half2*>(&h2);
 }
+__device__ __forceinline__ float2 from_e4m3x2(const unsigned codes) { return __half22float2(half_from_e4m3x2(codes)); }
 
 __device__ __forceinline__ float r8_widen(const float v) { return v; }
 __device__ __forceinline__ float r8_widen(const __half v) { return __half2float(v); }
@@ -94,17 +95,31 @@ __device__ __forceinline__ void r8_load8(const T* row, const int c, const int D,
 // squared norm.
 template <int G>
 __device__ __forceinline__ uint2 r8_quantise(float (&x)[8], unsigned& byte, float& part) {
-    unsigned top = 0u;                     // magnitudes of finite numbers order like their bits
+    unsigned top = 0u;                     // magnitudes order like their bits
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const unsigned m = __float_as_uint(x[k]) & 0x7fffffffu;
-        if (m >= 0x7f800000u) x[k] = __uint_as_float(0x7fc00000u);
-        else top = m > top ? m : top;
+        top = m > top ? m : top;
     }
 #pragma unroll
     for (int off = G / 2; off > 0; off >>= 1) {
         const unsigned o = __shfl_xor_sync(kFull, top, off);
         top = o > top ? o : top;
+    }
+    if (__any_sync(kFull, top >= 0x7f800000u)) {
+        // a NaN or an infinity somewhere in the warp's blocks: they become NaN and count for no maximum
+        top = 0u;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const unsigned m = __float_as_uint(x[k]) & 0x7fffffffu;
+            if (m >= 0x7f800000u) x[k] = __uint_as_float(0x7fc00000u);
+            else top = m > top ? m : top;
+        }
+#pragma unroll
+        for (int off = G / 2; off > 0; off >>= 1) {
+            const unsigned o = __shfl_xor_sync(kFull, top, off);
+            top = o > top ? o : top;
+        }
     }
     // amax = m * 2^E with 1 <= m < 2; 448 = 1.75 * 2^8
     int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
@@ -115,9 +130,9 @@ __device__ __forceinline__ uint2 r8_quantise(float (&x)[8], unsigned& byte, floa
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         q[k] = to_e4m3x2(mul_keep(x[2 * k], inv), mul_keep(x[2 * k + 1], inv));
-        const float2 v = from_e4m3x2(q[k]);
-        sum = __fmaf_rn(v.x, v.x, sum);
-        sum = __fmaf_rn(v.y, v.y, sum);
+        const __half2 v = half_from_e4m3x2(q[k]);          // (a half holds every code: the squares are exact)
+        sum = fma_half(__low2half(v), __low2half(v), sum);
+        sum = fma_half(__high2half(v), __high2half(v), sum);
     }
     byte = (unsigned)(e + 127);
     part = __fmul_rn(__fmul_rn(sum, scale), scale);
