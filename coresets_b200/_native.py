@@ -19,6 +19,7 @@ F_ELEMENT_ORDER = 1
 F_PDL = 2
 F_X_HALF = 4
 F_TEST_STALL_PIPE = 0x100
+ROWS8_TEST_STALL = 0x100
 CS_CTL_BYTES = 256
 CELL_TILE = 256
 CELLS_META_BYTES = 128
@@ -104,7 +105,7 @@ class CsRows8(ctypes.Structure):
         ("capacity", ctypes.c_int64),
         ("count", ctypes.c_int64),
         ("dim", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
     ]
 
 

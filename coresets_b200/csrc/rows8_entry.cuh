@@ -220,6 +220,8 @@ R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {
     j.D = lanes->dim;
     j.words = r8_words(lanes->dim);
     j.status = lanes->status;
+    j.stall = (lanes->flags & CS_ROWS8_TEST_STALL) != 0;
+    j.wait_ns = j.stall ? kR8TestWaitNs : kR8WaitNs;
     return j;
 }
 

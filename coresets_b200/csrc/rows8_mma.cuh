@@ -21,7 +21,8 @@ namespace {
 
 enum { R8_PRODUCTS = 0, R8_COVERAGE = 1 };
 constexpr int kR8Lanes = 128;                       // rows of the lane operand in a tile
-constexpr unsigned long long kR8WaitNs = 10000000000ull;      // the bound of every wait, that of the engine's pipes
+// The bound of every wait, that of the engine's pipes; short where a test makes one run out.
+constexpr unsigned long long kR8WaitNs = 10000000000ull, kR8TestWaitNs = 20000000ull;
 
 struct R8Job {
     const unsigned char* lane_scales;
@@ -38,6 +39,8 @@ struct R8Job {
     int bulk_out;                                   // products: out takes bulk stores
     int keep;                                       // coverage: min with what h holds
     int* status;
+    int stall;                                      // test hook: the producer starts no copy, so that the waits run out
+    unsigned long long wait_ns;
 };
 
 __device__ __forceinline__ uint64_t umma_desc(const uint32_t smem, const uint32_t stride_bytes, const uint64_t swizzle) {
@@ -96,28 +99,32 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
-// Wait that also ends when another role has given up.  The clock is looked at only after many tries (each
-// of which the hardware may itself hold for a while): reading it costs more than most waits last.
-__device__ __forceinline__ bool r8_wait(uint64_t* b, const uint32_t parity, volatile int* abort_flag) {
+// Wait that also ends when another role has given up.  The clock is looked at only after a number of tries
+// (each of which the hardware may itself hold for a while).
+struct R8Bound {
+    volatile int* abort_flag;
+    unsigned long long ns;
+};
+__device__ __forceinline__ bool r8_wait(uint64_t* b, const uint32_t parity, const R8Bound& bound) {
     if (mbar_try(b, parity)) return true;
     unsigned long long t0 = 0;
     for (;;) {
 #pragma unroll 1
-        for (int it = 0; it < 1024; ++it)
+        for (int it = 0; it < 64; ++it)
             if (mbar_try(b, parity)) return true;
-        if (*abort_flag) return false;
+        if (*bound.abort_flag) return false;
         const unsigned long long now = global_ns();
         if (t0 == 0) t0 = now;
-        if (now - t0 > kR8WaitNs) {
-            *abort_flag = 1;
+        if (now - t0 > bound.ns) {
+            *bound.abort_flag = 1;
             return false;
         }
     }
 }
 
 // the same by a whole converged warp
-__device__ __forceinline__ bool r8_wait_warp(uint64_t* b, const uint32_t parity, volatile int* abort_flag) {
-    return __all_sync(kFull, r8_wait(b, parity, abort_flag));
+__device__ __forceinline__ bool r8_wait_warp(uint64_t* b, const uint32_t parity, const R8Bound& bound) {
+    return __all_sync(kFull, r8_wait(b, parity, bound));
 }
 
 template <int NT, int WHAT, typename T> struct R8Shape {
@@ -142,7 +149,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_word;
     __shared__ __align__(16) float s_norm[4][NT < 32 ? 32 : NT];          // a copy per reading warp: no barrier between them
-    volatile int* s_abort = &s_abort_word;
+    const R8Bound s_abort{&s_abort_word, job.wait_ns};
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
 
     const int warp = __shfl_sync(kFull, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;    // warp: known to be uniform
@@ -165,7 +172,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
 
     if (warp == 0) {
         uint32_t n = 0;                                                // stages filled so far
-        bool ok = true;
+        bool ok = !job.stall;
         for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x) {
             for (int kb = 0; kb < kblocks; ++kb, ++n) {
                 const uint32_t st = n % S::kStages, round = n / S::kStages;

@@ -149,7 +149,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_word;
     __shared__ __align__(1024) unsigned char s_power[S::kNorms ? 4096 + 512 : 16];      // the lane operand of the norms' step, and its scales
-    volatile int* s_abort = &s_abort_word;
+    const R8Bound s_abort{&s_abort_word, job.wait_ns};
     unsigned char* kept = reinterpret_cast<unsigned char*>(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
     unsigned char* tiles = kept + S::kKept;
 
@@ -194,7 +194,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
     if (warp == 0) {
         uint32_t st = 0, phase = 0;
         uint32_t n = 0, items = 0;
-        bool ok = true;
+        bool ok = !job.stall;
         for (int64_t at = first; at < last && ok;) {
             const PairSpan sp = pair_span<S::kNorms>(job, at, last);
             at = sp.next;

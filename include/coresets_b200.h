@@ -404,6 +404,8 @@ CS_API int cs_fps_step_noalloc(const float* X, const float* norms, float* h, int
  * 16-byte aligned.  Rows < 2^31, dim <= CS_ROWS8_MAX_DIM.
  */
 #define CS_ROWS8_MAX_DIM 65536
+#define CS_ROWS8_TEST_STALL 0x100 /* test hook: a product over this store starts no copy, so that its bounded
+                              waits run out (20 ms, status 4) without any fault */
 #define CS_DTYPE_F32 0
 #define CS_DTYPE_F16 1
 #define CS_DTYPE_BF16 2
@@ -416,7 +418,7 @@ typedef struct cs_rows8 {
     int64_t capacity;    /* rows that the arrays hold                                                */
     int64_t count;       /* rows in use: what reads and products take                                 */
     int32_t dim;
-    int32_t reserved;
+    int32_t flags;       /* 0, or CS_ROWS8_TEST_STALL                                                   */
 } cs_rows8;
 
 /* Quantise n rows of X (dtype CS_DTYPE_*, row stride ld elements) into rows start .. start + n of the

@@ -5,7 +5,7 @@ import torch
 
 import coresets_b200 as coresets
 import oracle
-from coresets_b200 import RowStore, coverage, quantise_rows, read_rows, row_products
+from coresets_b200 import RowStore, _native, coverage, quantise_rows, read_rows, row_products
 from coresets_b200.rows8 import store_matrix
 from tests import rows8_oracle as ref
 from tests.data import gaussian_mixture
@@ -427,15 +427,41 @@ def test_refusals():
         coresets.fps_cuda(a, 3)
 
 
-def test_status_word_reaches_the_host():
-    a, b = quantise_rows(rows(4, 32).cuda()), quantise_rows(rows(4, 32).cuda())
-    row_products(a, b)
+@pytest.mark.parametrize("n,k", [(300, 5), (300, 200), (2000, 1000)])
+def test_a_wait_that_runs_out_sets_the_status(n, k):
+    """With the test hook the kernels' producer starts no copy: every wait ends by its bound, the block leaves, the status says
+    so, and the next calls work."""
+    a, c = quantise_rows(rows(n, 300, 1).cuda()), quantise_rows(rows(k, 300, 2).cuda())
+    want = row_products(a, c), coverage(a, c)
+    a._c.flags = c._c.flags = _native.ROWS8_TEST_STALL
+    for call in (row_products, coverage):
+        call(a, c)
+        with pytest.raises(RuntimeError, match="ran out"):
+            a.check_status()
+        a._status.zero_()
+    a._c.flags = c._c.flags = 0
+    assert torch.equal(row_products(a, c), want[0]) and torch.equal(coverage(a, c), want[1])
     a.check_status()
-    a._status.fill_(4)                                            # what a kernel leaves whose bounded wait ran out
-    with pytest.raises(RuntimeError, match="ran out"):
-        a.check_status()
     with pytest.raises(AttributeError):
-        a.codes = b.codes
+        a.codes = c.codes
+
+
+def test_calls_on_several_streams_at_once():
+    a, b, c = (quantise_rows(rows(n, 256, n).cuda()) for n in (20000, 3000, 600))
+    few = c.take(torch.arange(9))
+    calls = [lambda: coverage(a, c), lambda: row_products(b, c, dtype=torch.bfloat16), lambda: row_products(few, a), lambda: coverage(a, few),
+             lambda: read_rows(a), lambda: row_products(c, b)]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(10):
+        for f, s, g in zip(calls, streams, got):
+            with torch.cuda.stream(s):
+                g.append(f())
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
 
 
 def test_from_tensors_shares_memory():

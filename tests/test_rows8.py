@@ -53,7 +53,7 @@ def lib():
 
 
 def _store(**kw):
-    v = dict(codes=4096, scales=8192, norms=12288, status=None, capacity=100, count=50, dim=64, reserved=0)
+    v = dict(codes=4096, scales=8192, norms=12288, status=None, capacity=100, count=50, dim=64, flags=0)
     v.update(kw)
     return _native.CsRows8(*v.values())
 
