@@ -6,7 +6,7 @@
 namespace {
 
 int validate_rows8(const cs_rows8* r) {
-    if (!r || r->capacity < 0 || r->count < 0 || r->count > r->capacity || r->dim < 1) return CS_E_ARG;
+    if (!r || r->capacity < 0 || r->count < 0 || r->count > r->capacity || r->dim < 1 || (r->flags & ~CS_ROWS8_TEST_STALL)) return CS_E_ARG;
     if (r->capacity > 0 && (!r->codes || !r->scales || !r->norms)) return CS_E_ARG;
     if (r->capacity >= (int64_t)1 << 31 || r->dim > CS_ROWS8_MAX_DIM) return CS_E_RANGE;
     if (((uintptr_t)r->codes | (uintptr_t)r->scales | (uintptr_t)r->norms) & 15u) return CS_E_ALIGN;

@@ -67,7 +67,7 @@ def test_c_abi_refusals(lib):
     ARG, ALIGN, RANGE = -1, -2, -3
     r, p = ctypes.byref, 16384
     good = _store()
-    for bad, code in ((_store(dim=0), ARG), (_store(codes=None), ARG), (_store(count=101), ARG), (_store(capacity=-1, count=-1), ARG),
+    for bad, code in ((_store(dim=0), ARG), (_store(codes=None), ARG), (_store(count=101), ARG), (_store(capacity=-1, count=-1), ARG), (_store(flags=1), ARG),
                       (_store(norms=12290), ALIGN), (_store(scales=8200), ALIGN), (_store(capacity=2 ** 31), RANGE), (_store(dim=65537), RANGE)):
         assert lib.cs_rows8_write(r(bad), p, 0, 1, 64, 0, None) == code
         assert lib.cs_rows8_read(r(bad), p, 1, p, 0, 64, None) == code
