@@ -190,11 +190,11 @@ int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cu
     if (!rc && WHAT == R8_PRODUCTS) rc = r8_out_map<T>(&out_map, job, NT);
     if (rc) return rc;
     static thread_local KernelTune tune;
-    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, S::kSmem, 192, nullptr);
+    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, S::kSmem, S::kThreads, nullptr);
     if (rc) return rc;
     job.items = (job.n_lane + kR8Lanes - 1) / kR8Lanes;
     const int grid = (int)(job.items < d.sms ? job.items : d.sms);
-    rows8_mma_kernel<NT, WHAT, T><<<grid, 192, S::kSmem, st>>>(lane_map, col_map, out_map, job);
+    rows8_mma_kernel<NT, WHAT, T><<<grid, S::kThreads, S::kSmem, st>>>(lane_map, col_map, out_map, job);
     return check_launch();
 }
 // the narrowest tile that holds all columns; pairs of SMs where 64 do not (coverage of 1M x 128 by 8192 centres:

@@ -132,14 +132,20 @@ template <int NT, int WHAT, typename T> struct R8Shape {
     static constexpr int kStage = kTileA + kTileB + 1024;              // two tiles, two scale words of 128 rows
     static constexpr int kAcc = 256 / (NT < 32 ? 32 : NT);             // accumulators: 8, 8, 4; the way from a tile's last MMA to its
                                                                        // free accumulator is much longer than its few MMAs
+    // Sets of four reading warps (a set has the tile's 128 lanes), tile by tile in turn: a reader's way from accumulator to
+    // memory is long, and what a tile takes else is short (461k x 10 x 16 to float16: 39 us with one set, 34 with four; 1M x 64 x 128: coverage 49 -> 33).  kAcc
+    // is a multiple of it, so that the wait for an accumulator's fill comes after the same set's wait for the fill before.
+    static constexpr int kSets = kAcc / 2;
+    static constexpr int kThreads = 64 + 128 * kSets;
     static constexpr int kOutWarp = WHAT == R8_PRODUCTS ? (32 * (NT + 1) * (int)sizeof(T) + 127) & ~127 : 0;      // a reader's products on their way out
-    static constexpr int kOut = 4 * kOutWarp;
-    static constexpr int kStages = kOut > 16384 ? 7 : 8;
+    static constexpr int kOut = 4 * kSets * kOutWarp;
+    static constexpr int kFit = (226 * 1024 - kOut - 1024 - 2048) / kStage;
+    static constexpr int kStages = kFit < 8 ? kFit : 8;
     static constexpr int kSmem = kStages * kStage + kOut + 1024;       // slack to align the tiles to 1 KB
 };
 
 template <int NT, int WHAT, typename T>
-__global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant__ CUtensorMap lane_map,
+__global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma_kernel(const __grid_constant__ CUtensorMap lane_map,
                                                            const __grid_constant__ CUtensorMap col_map,
                                                            const __grid_constant__ CUtensorMap out_map, const R8Job job) {
     using S = R8Shape<NT, WHAT, T>;
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
     __shared__ uint64_t s_full[S::kStages], s_empty[S::kStages], s_acc_full[S::kAcc], s_acc_empty[S::kAcc];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_word;
-    __shared__ __align__(16) float s_norm[4][NT < 32 ? 32 : NT];          // a copy per reading warp: no barrier between them
+    __shared__ __align__(16) float s_norm[4 * S::kSets][NT < 32 ? 32 : NT];          // a copy per reading warp: no barrier between them
     const R8Bound s_abort{&s_abort_word, job.wait_ns};
     unsigned char* tiles = reinterpret_cast<unsigned char*>(((uintptr_t)s_raw + 1023) & ~(uintptr_t)1023);
 
@@ -230,18 +236,20 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
             for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n; ++k)
                 for (int it = 0; it < (1 << 16) && !mbar_try(&s_empty[k % S::kStages], (k / S::kStages) & 1u); ++it) {}
     } else {
-        const int quad = warp & 3;
+        const int quad = warp & 3, set = (warp - 2) >> 2, reader = warp - 2;
         const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
         uint32_t t = 0;
         bool ok = true;
         if (WHAT == R8_COVERAGE) {
             // the centres' norms; a column past the last centre can never be the nearest
-            for (int c = lane; c < NT; c += 32) s_norm[quad][c] = c < job.n_col ? __ldg(job.col_norms + c) : __uint_as_float(0x7f800000u);
+            for (int c = lane; c < NT; c += 32) s_norm[reader][c] = c < job.n_col ? __ldg(job.col_norms + c) : __uint_as_float(0x7f800000u);
             __syncwarp();
         }
         for (int64_t item = blockIdx.x; item < job.items && ok; item += gridDim.x, ++t) {
+            if (t % S::kSets != (uint32_t)set) continue;
             const int64_t row = item * kR8Lanes + quad * 32 + lane;
             const uint32_t buf = t % S::kAcc;
+            const float row_norm = WHAT == R8_COVERAGE && row < job.n_lane ? __ldg(job.lane_norms + row) : 0.0f;      // (ahead of the wait)
             ok = r8_wait_warp(&s_acc_full[buf], (t / S::kAcc) & 1u, s_abort);
             if (!ok) break;
             tc_fence_after();
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_acc_empty[buf]);
             if (WHAT == R8_PRODUCTS) {
-                T* mine = reinterpret_cast<T*>(tiles + S::kStages * S::kStage + quad * S::kOutWarp);
+                T* mine = reinterpret_cast<T*>(tiles + S::kStages * S::kStage + reader * S::kOutWarp);
                 if (job.bulk_out) {
                     // NT columns x 32 lanes through shared memory, one bulk store for the warp
                                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -303,8 +311,8 @@ __global__ void __launch_bounds__(192, 1) rows8_mma_kernel(const __grid_constant
 #pragma unroll
                 for (int j = 0; j < 4; ++j) best[j] = __uint_as_float(0x7f800000u);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) best[j & 3] = fminf(best[j & 3], __fmaf_rn(-2.0f, __uint_as_float(v[j]), s_norm[quad][j]));
-                const float d = __fadd_rn(__ldg(job.lane_norms + row), fminf(fminf(best[0], best[1]), fminf(best[2], best[3])));
+                for (int j = 0; j < NT; ++j) best[j & 3] = fminf(best[j & 3], __fmaf_rn(-2.0f, __uint_as_float(v[j]), s_norm[reader][j]));
+                const float d = __fadd_rn(row_norm, fminf(fminf(best[0], best[1]), fminf(best[2], best[3])));
                 const float up = d == d ? fmaxf(d, 0.0f) : __uint_as_float(0x7f800000u);
                 float* h = reinterpret_cast<float*>(job.out) + row;
                 *h = job.keep ? fminf(*h, up) : up;

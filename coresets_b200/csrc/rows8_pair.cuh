@@ -327,6 +327,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             at = sp.next;
             const int64_t row = sp.lt * kPairLanes + rank * kR8Lanes + quad * 32 + lane;
             float best[4] = {low, low, low, low};
+            const float row_norm = WHAT == R8_COVERAGE && row < job.n_lane ? __ldg(job.lane_norms + row) : 0.0f;     // (ahead of the tiles)
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct, ++t) {
                 const uint32_t buf = t & 1u;
                 ok = r8_wait_warp(&s_acc_full[buf], (t >> 1) & 1u, s_abort);
@@ -371,7 +372,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             }
             if (WHAT == R8_COVERAGE && ok && row < job.n_lane) {
                 // |a - c|^2 = |a|^2 - 2 (a.c - |c|^2 / 2)
-                const float d = __fmaf_rn(-2.0f, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])), __ldg(job.lane_norms + row));
+                const float d = __fmaf_rn(-2.0f, fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])), row_norm);
                 if (d == d)      // h holds +inf or what it had: a NaN leaves that; max(d, 0) orders like its bits
                     atomicMin(reinterpret_cast<int*>(job.out) + row, __float_as_int(fmaxf(d, 0.0f)));
             }
