@@ -95,16 +95,22 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
+// Bytes of a row in a tile: the narrowest swizzle that holds the row, 128 (a block) where none does.  A copy that is mostly
+// past the end of its rows is slow, as is one that L2 widens past them (coverage of 1M x 16 by 576: 208 us with 128 bytes a row
+// and 256 at a time from L2, 96 this way; by 16: 87 and 56).
+int r8_width_of(const int dim) { return dim <= 16 ? 16 : (dim <= 32 ? 32 : (dim <= 64 ? 64 : kR8Block)); }
+
 // rows of `dim` bytes as tiles of `rows` x `width`; what lies behind the last row or the pitch reads as 0
-int r8_map(CUtensorMap* map, void* base, const int dim, const int64_t count, const int width, const int rows, const bool swizzle) {
+int r8_map(CUtensorMap* map, void* base, const int dim, const int64_t count, const int width, const int rows) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return CS_E_DEVICE;
     const cuuint64_t dims[2] = {(cuuint64_t)r8_pitch(dim), (cuuint64_t)count};
     const cuuint64_t strides[1] = {(cuuint64_t)r8_pitch(dim)};
     const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)rows}, step[2] = {1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+    const CUtensorMapSwizzle swizzle = width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B :
+                                       (width == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE));
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? CS_OK
                : CS_E_ARG;
 }
@@ -145,12 +151,12 @@ int r8_out_map(CUtensorMap* map, R8Job& job, const int cols) {
 // what the pair kernel's extra step needs per column, rounded up to whole tiles: 16 bytes of digits, then scale words
 int64_t r8_norm_rows(const int64_t n_col) { return n_col <= 64 ? 0 : (n_col + kPairCols - 1) / kPairCols * kPairCols; }
 
-template <int WHAT, typename T, bool KEEP>
+template <int WHAT, typename T, bool KEEP, bool NARROW>
 int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, void* work, cudaStream_t st, const DevInfo& d) {
     using S = PairShape<WHAT, T, KEEP>;
     PairMaps maps = {};
-    int rc = r8_map(&maps.lane, lanes->codes, lanes->dim, lanes->count, kR8Block, kR8Lanes, true);
-    if (!rc) rc = r8_map(&maps.col, cols->codes, cols->dim, cols->count, kR8Block, kPairCols / 2, true);
+    int rc = r8_map(&maps.lane, lanes->codes, lanes->dim, lanes->count, job.width, kR8Lanes);
+    if (!rc) rc = r8_map(&maps.col, cols->codes, cols->dim, cols->count, job.width, kPairCols / 2);
     if (!rc) rc = r8_scale_map(&maps.lane_sf, lanes->scales, lanes->dim, lanes->count, 1);
     if (!rc) rc = r8_scale_map(&maps.col_sf, cols->scales, cols->dim, cols->count, 2);
     if (rc) return rc;
@@ -165,7 +171,7 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
         rows8_norm_digits_kernel<<<r8_grid((most + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(job.col_norms, job.n_col, rows, digits, scales,
                                                                                                  static_cast<float*>(job.out), n_h);
         rc = check_launch();
-        if (!rc) rc = r8_map(&maps.norm, digits, 16, rows, 16, kPairCols / 2, false);
+        if (!rc) rc = r8_map(&maps.norm, digits, 16, rows, 16, kPairCols / 2);
         if (!rc) rc = r8_scale_map(&maps.norm_sf, scales, 1, rows, 2);
         if (rc) return rc;
     }
@@ -174,28 +180,33 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
         if (rc) return rc;
     }
     static thread_local KernelTune tune;
-    rc = tune_kernel(rows8_pair_kernel<WHAT, T, KEEP>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
+    rc = tune_kernel(rows8_pair_kernel<WHAT, T, KEEP, NARROW>, tune, d.dev, S::kSmem, kPairWarps * 32, nullptr);
     if (rc) return rc;
     const int grid = 2 * (int)(job.tiles < pairs ? job.tiles : pairs);
-    rows8_pair_kernel<WHAT, T, KEEP><<<grid, kPairWarps * 32, S::kSmem, st>>>(maps, job);
+    rows8_pair_kernel<WHAT, T, KEEP, NARROW><<<grid, kPairWarps * 32, S::kSmem, st>>>(maps, job);
     return check_launch();
 }
 
-template <int NT, int WHAT, typename T>
-int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
+template <int NT, int WHAT, typename T, bool NARROW>
+int launch_rows8_mma_width(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
     using S = R8Shape<NT, WHAT, T>;
     CUtensorMap lane_map, col_map, out_map = {};
-    int rc = r8_map(&lane_map, lanes->codes, lanes->dim, lanes->count, kR8Block, kR8Lanes, true);
-    if (!rc) rc = r8_map(&col_map, cols->codes, cols->dim, cols->count, kR8Block, NT, true);
+    int rc = r8_map(&lane_map, lanes->codes, lanes->dim, lanes->count, job.width, kR8Lanes);
+    if (!rc) rc = r8_map(&col_map, cols->codes, cols->dim, cols->count, job.width, NT);
     if (!rc && WHAT == R8_PRODUCTS) rc = r8_out_map<T>(&out_map, job, NT);
     if (rc) return rc;
     static thread_local KernelTune tune;
-    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T>, tune, d.dev, S::kSmem, S::kThreads, nullptr);
+    rc = tune_kernel(rows8_mma_kernel<NT, WHAT, T, NARROW>, tune, d.dev, S::kSmem, S::kThreads, nullptr);
     if (rc) return rc;
     job.items = (job.n_lane + kR8Lanes - 1) / kR8Lanes;
     const int grid = (int)(job.items < d.sms ? job.items : d.sms);
-    rows8_mma_kernel<NT, WHAT, T><<<grid, S::kThreads, S::kSmem, st>>>(lane_map, col_map, out_map, job);
+    rows8_mma_kernel<NT, WHAT, T, NARROW><<<grid, S::kThreads, S::kSmem, st>>>(lane_map, col_map, out_map, job);
     return check_launch();
+}
+template <int NT, int WHAT, typename T>
+int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, cudaStream_t st, const DevInfo& d) {
+    return job.width < kR8Block ? launch_rows8_mma_width<NT, WHAT, T, true>(lanes, cols, job, st, d)
+                                : launch_rows8_mma_width<NT, WHAT, T, false>(lanes, cols, job, st, d);
 }
 // the narrowest tile that holds all columns; pairs of SMs where 64 do not (coverage of 1M x 128 by 8192 centres:
 // 1.28 ms, with tiles of 128 x 128 on single SMs 3.11 ms)
@@ -205,8 +216,9 @@ int launch_rows8_mma(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, vo
     if (job.n_col <= 32) return launch_rows8_mma<32, WHAT, T>(lanes, cols, job, st, d);
     if (job.n_col <= 64) return launch_rows8_mma<64, WHAT, T>(lanes, cols, job, st, d);
     constexpr bool kMayKeep = WHAT == R8_COVERAGE;
-    if (kMayKeep && job.D <= kPairKept * kR8Block) return launch_rows8_pair<WHAT, T, kMayKeep>(lanes, cols, job, work, st, d);
-    return launch_rows8_pair<WHAT, T, false>(lanes, cols, job, work, st, d);
+    if (job.width < kR8Block) return launch_rows8_pair<WHAT, T, kMayKeep, true>(lanes, cols, job, work, st, d);
+    if (kMayKeep && job.D <= kPairKept * kR8Block) return launch_rows8_pair<WHAT, T, kMayKeep, false>(lanes, cols, job, work, st, d);
+    return launch_rows8_pair<WHAT, T, false, false>(lanes, cols, job, work, st, d);
 }
 
 R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {
@@ -219,6 +231,7 @@ R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {
     j.n_col = cols->count;
     j.D = lanes->dim;
     j.words = r8_words(lanes->dim);
+    j.width = r8_width_of(lanes->dim);
     j.status = lanes->status;
     j.stall = (lanes->flags & CS_ROWS8_TEST_STALL) != 0;
     j.wait_ns = j.stall ? kR8TestWaitNs : kR8WaitNs;

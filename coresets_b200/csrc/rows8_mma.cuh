@@ -31,6 +31,7 @@ struct R8Job {
     const float* col_norms;
     int64_t n_lane, n_col;                          // rows of the two operands
     int D, words;
+    int width;                                      // bytes of a row in a tile: 16, 32, 64 or 128 (a block of 128, or the whole row)
     int col_tiles;                                  // rows8_pair.cuh: column tiles, and tiles in all
     int64_t tiles;
     int64_t items;                                  // here: lane tiles (one tile holds all columns)
@@ -47,6 +48,15 @@ __device__ __forceinline__ uint64_t umma_desc(const uint32_t smem, const uint32_
     // start >> 4, stride between the 16-byte halves of a step's codes >> 4 (1; unused with a swizzle), stride
     // between groups of 8 rows >> 4, the constant 1 of this architecture, swizzle mode
     return (uint64_t)((smem & 0x3ffffu) >> 4) | (1ull << 16) | ((uint64_t)(stride_bytes >> 4) << 32) | (1ull << 46) | (swizzle << 61);
+}
+// Codes of a tile: rows of `width` bytes, swizzled over that width (16: not swizzled, and the step's second 16 codes are
+// `lbo` bytes further on, where the tile holds zeros).
+__device__ __forceinline__ uint64_t tile_desc(const uint32_t smem, const int width, const uint32_t lbo) {
+    const uint64_t d = umma_desc(smem, 8u * (uint32_t)width, width == 128 ? 2u : (width == 64 ? 4u : (width == 32 ? 6u : 0u)));
+    return width == 16 ? d + ((uint64_t)((lbo >> 4) - 1u) << 16) : d;
+}
+__device__ __forceinline__ void zero_smem(unsigned char* p, const int bytes) {
+    for (int i = 16 * (int)threadIdx.x; i < bytes; i += 16 * (int)blockDim.x) *reinterpret_cast<uint4*>(p + i) = make_uint4(0u, 0u, 0u, 0u);
 }
 __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, const int x, const int y, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -144,7 +154,8 @@ template <int NT, int WHAT, typename T> struct R8Shape {
     static constexpr int kSmem = kStages * kStage + kOut + 1024;       // slack to align the tiles to 1 KB
 };
 
-template <int NT, int WHAT, typename T>
+// NARROW: rows of at most 64 codes (one step or two of the MMA), tiles of job.width bytes a row.
+template <int NT, int WHAT, typename T, bool NARROW>
 __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma_kernel(const __grid_constant__ CUtensorMap lane_map,
                                                            const __grid_constant__ CUtensorMap col_map,
                                                            const __grid_constant__ CUtensorMap out_map, const R8Job job) {
@@ -166,6 +177,14 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
         for (int i = 0; i < S::kAcc; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 4); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    const int width = NARROW ? job.width : kR8Block;
+    if (NARROW && width == 16) {
+        for (int i = 0; i < S::kStages; ++i) {
+            zero_smem(tiles + i * S::kStage + kR8Lanes * 64, kR8Lanes * 16);
+            zero_smem(tiles + i * S::kStage + S::kTileA + NT * 64, NT * 16);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -185,7 +204,7 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                 if (round > 0 && !r8_wait_warp(&s_empty[st], (round - 1) & 1u, s_abort)) { ok = false; break; }
                 unsigned char* a = tiles + st * S::kStage;
                 if (elect_one()) {
-                    mbar_expect_tx(&s_full[st], S::kStage);
+                    mbar_expect_tx(&s_full[st], (uint32_t)((kR8Lanes + NT) * width + 1024));
                     tma_tile(a, &lane_map, kb * kR8Block, (int)(item * kR8Lanes), &s_full[st]);
                     tma_tile(a + S::kTileA, &col_map, kb * kR8Block, 0, &s_full[st]);
                     bulk_load(a + S::kTileA + S::kTileB, job.lane_scales + (item * job.words + (kb >> 2)) * 512, 512, &s_full[st]);
@@ -222,9 +241,13 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                     tc_copy_scales(sfb, umma_desc(sf + 512, 128, 0));
                     const uint32_t id = kIdesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
                     const int left = job.D - kb * kR8Block, steps = left >= kR8Block ? 4 : (left + 31) >> 5;
-                    const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
-                    for (int k = 0; k < steps; ++k)
-                        tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, kb > 0 || k > 0);
+                    if constexpr (!NARROW) {
+                        const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
+                        for (int k = 0; k < steps; ++k) tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, kb > 0 || k > 0);
+                    } else {
+                        const uint64_t da = tile_desc(a, width, kR8Lanes * 64), db = tile_desc(b, width, NT * 64);
+                        for (int k = 0; k < steps; ++k) tc_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb, k > 0);
+                    }
                     tc_commit(&s_empty[st]);
                     if (kb == kblocks - 1) tc_commit(&s_acc_full[buf]);
                 }

@@ -139,7 +139,7 @@ __device__ __forceinline__ PairSpan pair_span(const R8Job& job, const int64_t at
 
 struct PairMaps { CUtensorMap lane, col, lane_sf, col_sf, norm, norm_sf, out; };
 
-template <int WHAT, typename T, bool KEEP>
+template <int WHAT, typename T, bool KEEP, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairWarps * 32, 1)
 rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
     using S = PairShape<WHAT, T, KEEP>;
@@ -180,6 +180,16 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             *reinterpret_cast<unsigned*>(tiles + kStages * S::kTile + (threadIdx.x >> 2) * S::kFirst + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    const int width = NARROW ? job.width : kR8Block;
+    if (NARROW && width == 16) {
+        if (KEEP)
+            for (int i = 0; i < 2; ++i) zero_smem(kept + i * (kPairKept / 2) * kPairA + kR8Lanes * 64, kR8Lanes * 16);
+        for (int i = 0; i < kStages; ++i) {
+            if (!KEEP) zero_smem(tiles + i * S::kTile + kR8Lanes * 64, kR8Lanes * 16);
+            zero_smem(tiles + (i + 1) * S::kTile - kPairB + kPairCols / 2 * 64, kPairCols / 2 * 16);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s_tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -204,7 +214,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                 if (round > 0 && !r8_wait_warp(&s_kept_empty[slot], (round - 1) & 1u, s_abort)) { ok = false; break; }
                 const uint32_t bar = leader_addr(&s_kept_full[slot]), to = smem_u32(kept) + slot * (kPairKept / 2) * kPairA;
                 if (elect_one()) {
-                    if (rank == 0) mbar_expect_tx(&s_kept_full[slot], 2 * kblocks * kPairA);
+                    if (rank == 0) mbar_expect_tx(&s_kept_full[slot], 2 * kblocks * kR8Lanes * width);
                     for (int kb = 0; kb < kblocks; ++kb) pair_tile(to + kb * kPairA, &maps.lane, kb * kR8Block, row, bar);
                 }
                 __syncwarp();
@@ -216,7 +226,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     const uint32_t a = smem_u32(tiles + st * S::kTile), sf = smem_u32(tiles + kStages * S::kTile + st * S::kFirst), bar = leader_addr(&s_full[st]);
                     const bool scales = (kb & 3) == 0;
                     if (elect_one()) {
-                        if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (S::kTile + (scales ? kPairSf : 0) + (S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0)));
+                        if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (((KEEP ? 0 : kR8Lanes) + kPairCols / 2) * width + (scales ? kPairSf : 0) + (S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0)));
                         if (!KEEP) pair_tile(a, &maps.lane, kb * kR8Block, row, bar);
                         pair_tile(a + S::kTile - kPairB, &maps.col, kb * kR8Block, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
                         if (scales) {
@@ -283,13 +293,19 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                             }
                             const uint32_t id = kIdesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
                             const int left = job.D - kb * kR8Block;
-                            const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
-                            if (left > 96) {
+                            // (NARROW kernels of their own: descriptors that the compiler knows but for the address issue 10 % faster)
+                            if constexpr (!NARROW) {
+                                const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
+                                if (left > 96) {
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
+                                    for (int k = 0; k < 4; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
+                                } else {
+                                    const int steps = (left + 31) >> 5;
+                                    for (int k = 0; k < steps; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
+                                }
                             } else {
-                                const int steps = (left + 31) >> 5;
-                                for (int k = 0; k < steps; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
+                                const uint64_t da = tile_desc(a, width, kR8Lanes * 64), db = tile_desc(b, width, kPairCols / 2 * 64);
+                                for (int k = 0; k < (left + 31) >> 5; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, k > 0);
                             }
                             if (S::kNorms && kb == 0) {
                                 // 16 of the step's 32 codes count (the lane operand's others are 0): as the second
