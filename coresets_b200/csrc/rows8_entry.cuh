@@ -95,10 +95,13 @@ EncodeTiled encode_tiled() {
     return fn;
 }
 
+constexpr int64_t kR8LineRows = ((int64_t)1 << 30) - 1024;
+
 // Bytes of a row in a tile: the narrowest swizzle that holds the row, 128 (a block) where none does.  A copy that is mostly
 // past the end of its rows is slow, as is one that L2 widens past them (coverage of 1M x 16 by 576: 208 us with 128 bytes a row
-// and 256 at a time from L2, 96 this way; by 16: 87 and 56).
-int r8_width_of(const int dim) { return dim <= 16 ? 16 : (dim <= 32 ? 32 : (dim <= 64 ? 64 : kR8Block)); }
+// and 256 at a time from L2, 96 this way; by 16: 87 and 30).
+// (16: as one sequence, whose places in units of 8 bytes have to fit 31 bits)
+int r8_width_of(const int dim, const int64_t rows) { return dim <= 16 && rows <= kR8LineRows ? 16 : (dim <= 32 ? 32 : (dim <= 64 ? 64 : kR8Block)); }
 
 // rows of `dim` bytes as tiles of `rows` x `width`; what lies behind the last row or the pitch reads as 0
 int r8_map(CUtensorMap* map, void* base, const int dim, const int64_t count, const int width, const int rows) {
@@ -107,8 +110,16 @@ int r8_map(CUtensorMap* map, void* base, const int dim, const int64_t count, con
     const cuuint64_t dims[2] = {(cuuint64_t)r8_pitch(dim), (cuuint64_t)count};
     const cuuint64_t strides[1] = {(cuuint64_t)r8_pitch(dim)};
     const cuuint32_t box[2] = {(cuuint32_t)width, (cuuint32_t)rows}, step[2] = {1, 1};
+    if (width == 16) {                                      // rows of 16 bytes, without a swizzle: one sequence, in units of 8 bytes
+        const cuuint64_t all[1] = {(cuuint64_t)count * 2};
+        const cuuint32_t part[1] = {(cuuint32_t)rows * 2};
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 1, base, all, strides, part, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+                   ? CS_OK
+                   : CS_E_ARG;
+    }
     const CUtensorMapSwizzle swizzle = width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : (width == 64 ? CU_TENSOR_MAP_SWIZZLE_64B :
-                                       (width == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE));
+                                       CU_TENSOR_MAP_SWIZZLE_32B);
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
                ? CS_OK
@@ -231,7 +242,7 @@ R8Job r8_job(const cs_rows8* lanes, const cs_rows8* cols) {
     j.n_col = cols->count;
     j.D = lanes->dim;
     j.words = r8_words(lanes->dim);
-    j.width = r8_width_of(lanes->dim);
+    j.width = r8_width_of(lanes->dim, lanes->count > cols->count ? lanes->count : cols->count);
     j.status = lanes->status;
     j.stall = (lanes->flags & CS_ROWS8_TEST_STALL) != 0;
     j.wait_ns = j.stall ? kR8TestWaitNs : kR8WaitNs;
@@ -323,6 +334,7 @@ int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int3
     rc = validate_rows8(centres);
     if (rc) return rc;
     if (a->dim != centres->dim) return CS_E_ARG;
+    if (centres->count > kR8LineRows) return CS_E_RANGE;
     if (a->count == 0) return CS_OK;
     if (!h) return CS_E_ARG;
     if ((uintptr_t)h & 3u) return CS_E_ALIGN;

@@ -62,6 +62,11 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, cons
     asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
 }
+// rows of 16 bytes are one sequence in memory and in the tile: x in units of 8 bytes
+__device__ __forceinline__ void tma_line(void* dst, const CUtensorMap* map, const int x, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.1d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2}], [%3];"
+                 ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(smem_u32(bar)) : "memory");
+}
 // one bulk store, from shared memory, of a box of the map's; what of it lies past the last row or column is left out
 __device__ __forceinline__ void r8_store_tile(const CUtensorMap* map, const int x, const int y, const uint32_t smem) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
@@ -205,8 +210,13 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                 unsigned char* a = tiles + st * S::kStage;
                 if (elect_one()) {
                     mbar_expect_tx(&s_full[st], (uint32_t)((kR8Lanes + NT) * width + 1024));
-                    tma_tile(a, &lane_map, kb * kR8Block, (int)(item * kR8Lanes), &s_full[st]);
-                    tma_tile(a + S::kTileA, &col_map, kb * kR8Block, 0, &s_full[st]);
+                    if (NARROW && width == 16) {
+                        tma_line(a, &lane_map, (int)(item * kR8Lanes * 2), &s_full[st]);
+                        tma_line(a + S::kTileA, &col_map, 0, &s_full[st]);
+                    } else {
+                        tma_tile(a, &lane_map, kb * kR8Block, (int)(item * kR8Lanes), &s_full[st]);
+                        tma_tile(a + S::kTileA, &col_map, kb * kR8Block, 0, &s_full[st]);
+                    }
                     bulk_load(a + S::kTileA + S::kTileB, job.lane_scales + (item * job.words + (kb >> 2)) * 512, 512, &s_full[st]);
                     bulk_load(a + S::kTileA + S::kTileB + 512, job.col_scales + (kb >> 2) * 512, 512, &s_full[st]);
                 }

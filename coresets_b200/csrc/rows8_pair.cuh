@@ -63,6 +63,11 @@ __device__ __forceinline__ void pair_tile(const uint32_t dst, const CUtensorMap*
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// rows of 16 bytes: one sequence (see tma_line)
+__device__ __forceinline__ void pair_line(const uint32_t dst, const CUtensorMap* map, const int x, const uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.1d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2}], [%3];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void pair_scales(const uint32_t dst, const CUtensorMap* map, const int w, const int chunk, const uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(0), "r"(w), "r"(chunk), "r"(bar) : "memory");
@@ -215,7 +220,9 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                 const uint32_t bar = leader_addr(&s_kept_full[slot]), to = smem_u32(kept) + slot * (kPairKept / 2) * kPairA;
                 if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(&s_kept_full[slot], 2 * kblocks * kR8Lanes * width);
-                    for (int kb = 0; kb < kblocks; ++kb) pair_tile(to + kb * kPairA, &maps.lane, kb * kR8Block, row, bar);
+                    if (NARROW && width == 16) pair_line(to, &maps.lane, 2 * row, bar);
+                    else
+                        for (int kb = 0; kb < kblocks; ++kb) pair_tile(to + kb * kPairA, &maps.lane, kb * kR8Block, row, bar);
                 }
                 __syncwarp();
                 ++items;
@@ -227,14 +234,20 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                     const bool scales = (kb & 3) == 0;
                     if (elect_one()) {
                         if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (((KEEP ? 0 : kR8Lanes) + kPairCols / 2) * width + (scales ? kPairSf : 0) + (S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0)));
-                        if (!KEEP) pair_tile(a, &maps.lane, kb * kR8Block, row, bar);
-                        pair_tile(a + S::kTile - kPairB, &maps.col, kb * kR8Block, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
+                        const int col = ct * kPairCols + (int)rank * (kPairCols / 2);
+                        if (NARROW && width == 16) {
+                            if (!KEEP) pair_line(a, &maps.lane, 2 * row, bar);
+                            pair_line(a + S::kTile - kPairB, &maps.col, 2 * col, bar);
+                        } else {
+                            if (!KEEP) pair_tile(a, &maps.lane, kb * kR8Block, row, bar);
+                            pair_tile(a + S::kTile - kPairB, &maps.col, kb * kR8Block, col, bar);
+                        }
                         if (scales) {
                             pair_scales(sf, &maps.lane_sf, kb >> 2, row >> 7, bar);
                             pair_scales(sf + 512, &maps.col_sf, kb >> 2, ct * kPairCols >> 7, bar);
                         }
                         if (S::kNorms && kb == 0) {
-                            pair_tile(sf + kPairSf + kPairNormSf, &maps.norm, 0, ct * kPairCols + (int)rank * (kPairCols / 2), bar);
+                            pair_line(sf + kPairSf + kPairNormSf, &maps.norm, 2 * col, bar);
                             pair_scales(sf + kPairSf, &maps.norm_sf, 0, ct * kPairCols >> 7, bar);
                         }
                     }

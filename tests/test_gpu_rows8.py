@@ -202,7 +202,7 @@ def product_bound(a, b, dtype):
 
 @pytest.mark.parametrize("n,k,dim", [
     (1, 1, 1), (1, 1, 128), (1, 300, 64), (300, 1, 64), (5, 16, 50), (16, 5, 50), (17, 33, 128), (33, 17, 129), (64, 200, 256), (200, 64, 256),
-    (65, 66, 100), (128, 128, 512), (129, 127, 513), (130, 1000, 1024), (1000, 130, 31), (777, 409, 1100), (3, 2000, 2050), (500, 140, 32), (260, 257, 96),
+    (65, 66, 100), (300, 300, 16), (400, 70, 13), (70, 400, 48), (500, 20, 16), (20, 500, 9), (300, 200, 24), (130, 129, 64), (128, 128, 512), (129, 127, 513), (130, 1000, 1024), (1000, 130, 31), (777, 409, 1100), (3, 2000, 2050), (500, 140, 32), (260, 257, 96),
 ])
 def test_products(n, k, dim):
     a, av = stored(n, dim, 3)
@@ -320,7 +320,7 @@ def coverage_bound(a, c, dim):
 
 
 @pytest.mark.parametrize("n,k,dim", [
-    (1, 1, 1), (1, 700, 128), (33, 2000, 128), (130, 16, 50), (128, 17, 64), (1000, 33, 100), (1000, 64, 256), (500, 65, 129), (300, 400, 513),
+    (1, 1, 1), (1, 700, 128), (33, 2000, 128), (130, 16, 50), (128, 17, 64), (1000, 33, 100), (1000, 64, 256), (700, 300, 16), (700, 300, 3), (500, 20, 16), (500, 90, 30), (500, 200, 48), (500, 65, 129), (300, 400, 513),
     (2000, 129, 31), (257, 300, 1024), (60, 50, 1100), (20000, 512, 64),
 ])
 def test_coverage(n, k, dim):

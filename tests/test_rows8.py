@@ -90,6 +90,7 @@ def test_c_abi_refusals(lib):
     assert lib.cs_rows8_coverage(r(good), r(good), p + 2, 0, None, None) == ALIGN
     many = _store(codes=40960, scales=81920, count=100)
     assert lib.cs_rows8_coverage_bytes(64) == 0 and lib.cs_rows8_coverage_bytes(100) >= 20 * 100 and lib.cs_rows8_coverage_bytes(-1) == ARG
+    assert lib.cs_rows8_coverage(r(good), r(_store(capacity=2 ** 30, count=2 ** 30)), p, 0, p, None) == RANGE
     # nothing to do
     none = _store(count=0)
     assert lib.cs_rows8_write(r(good), None, 0, 0, 64, 100, None) == 0
