@@ -306,27 +306,28 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                             }
                             const uint32_t id = kIdesc | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
                             const int left = job.D - kb * kR8Block;
+                            if (S::kNorms && kb == 0) {
+                                // first: the sums that follow pass through 0 instead of growing to |a| |c|, and the accumulator
+                                // loses less.  16 of the step's 32 codes count (the lane operand's others are 0): as the second 16 of
+                                // a row the descriptor names the next row's digits, then the zero bytes
+                                pair_copy_scales(sfb + 8, umma_desc(norm, 128, 0));
+                                pair_copy_scales(sfb + 12, umma_desc(norm + 512, 128, 0));
+                                pair_mma(acc, umma_desc(power, 128, 0) + (127ull << 16), umma_desc(norm + kPairNormSf, 128, 0), kIdesc, sf_power,
+                                         sfb + 8 + sub, false);
+                            }
                             // (NARROW kernels of their own: descriptors that the compiler knows but for the address issue 10 % faster)
                             if constexpr (!NARROW) {
                                 const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
                                 if (left > 96) {
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
+                                    for (int k = 0; k < 4; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || kb > 0 || k > 0);
                                 } else {
                                     const int steps = (left + 31) >> 5;
-                                    for (int k = 0; k < steps; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, kb > 0 || k > 0);
+                                    for (int k = 0; k < steps; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || kb > 0 || k > 0);
                                 }
                             } else {
                                 const uint64_t da = tile_desc(a, width, kR8Lanes * 64), db = tile_desc(b, width, kPairCols / 2 * 64);
-                                for (int k = 0; k < (left + 31) >> 5; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, k > 0);
-                            }
-                            if (S::kNorms && kb == 0) {
-                                // 16 of the step's 32 codes count (the lane operand's others are 0): as the second
-                                // 16 of a row the descriptor names the next row's digits, then the zero bytes
-                                pair_copy_scales(sfb + 8, umma_desc(norm, 128, 0));
-                                pair_copy_scales(sfb + 12, umma_desc(norm + 512, 128, 0));
-                                pair_mma(acc, umma_desc(power, 128, 0) + (127ull << 16), umma_desc(norm + kPairNormSf, 128, 0), kIdesc, sf_power,
-                                         sfb + 8 + sub, true);
+                                for (int k = 0; k < (left + 31) >> 5; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || k > 0);
                             }
                             pair_commit(&s_empty[st]);
                             if (kb == kblocks - 1) pair_commit(&s_acc_full[buf]);
