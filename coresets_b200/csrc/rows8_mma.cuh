@@ -67,11 +67,21 @@ __device__ __forceinline__ void tma_line(void* dst, const CUtensorMap* map, cons
     asm volatile("cp.async.bulk.tensor.1d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2}], [%3];"
                  ::"r"(smem_u32(dst)), "l"(map), "r"(x), "r"(smem_u32(bar)) : "memory");
 }
-// one bulk store, from shared memory, of a box of the map's; what of it lies past the last row or column is left out
+// One bulk store, from shared memory, of a box of the map's; what of it lies past the last row or column is left out.
+// Results are marked as the first to leave L2, for the operands' sake (4096 x 100 000 x 128 to bfloat16: 192 -> 172 us,
+// 20 000 x 20 000 x 128 to float32: 362 -> 343).
 __device__ __forceinline__ void r8_store_tile(const CUtensorMap* map, const int x, const int y, const uint32_t smem) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
-                 ::"l"(map), "r"(x), "r"(y), "r"(smem) : "memory");
+    unsigned long long policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group.L2::cache_hint [%0, {%1, %2}], [%3], %4;"
+                 ::"l"(map), "r"(x), "r"(y), "r"(smem), "l"(policy) : "memory");
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// one element of a result, likewise
+__device__ __forceinline__ void r8_put(float* p, const float v) { __stcs(p, v); }
+template <typename T>
+__device__ __forceinline__ void r8_put(T* p, const T v) {
+    __stcs(reinterpret_cast<unsigned short*>(p), *reinterpret_cast<const unsigned short*>(&v));
 }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -326,7 +336,7 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                             at[u] = r * job.lane_stride + c;
                         }
 #pragma unroll
-                        for (int u = 0; u < 8; ++u) out[at[u]] = o[u];
+                        for (int u = 0; u < 8; ++u) r8_put(out + at[u], o[u]);
                     }
                 } else if (row < job.n_lane) {
                     T* out = reinterpret_cast<T*>(job.out) + row * job.lane_stride;
@@ -335,7 +345,7 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                         if (j < job.n_col) {
                             T o;
                             r8_narrow(o, __uint_as_float(v[j]));
-                            out[j * job.col_stride] = o;
+                            r8_put(out + j * job.col_stride, o);
                         }
                 }
             } else if (row < job.n_lane) {

@@ -391,7 +391,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                             if (col + j < job.n_col) {
                                 T o;
                                 r8_narrow(o, __uint_as_float(v[j]));
-                                out[j * job.col_stride] = o;
+                                r8_put(out + j * job.col_stride, o);
                             }
                     }
                 } else {
