@@ -43,7 +43,9 @@ template <int WHAT, typename T, bool KEEP> struct PairShape {
 };
 static_assert(PairShape<R8_COVERAGE, float, true>::kSmem + 8192 <= 232448 && PairShape<R8_PRODUCTS, __half, false>::kSmem + 512 <= 232448 &&
               PairShape<R8_PRODUCTS, float, false>::kSmem + 512 <= 232448, "shared memory");
-static_assert(2 * kPairCols + 6 * 20 + 4 <= 512 && 2 * kPairCols + 6 * 12 <= 512, "TMEM columns");
+// behind the accumulators and the slots: the scales of the norms' lane operand, 4 columns for each issuing warp.  Copies and MMAs of
+// one thread keep their order, those of two do not: no warp writes columns that the other's MMAs read.
+static_assert(2 * kPairCols + 6 * 20 + 2 * 4 <= 512 && 2 * kPairCols + 6 * 12 <= 512, "TMEM columns");
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -271,7 +273,7 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             uint32_t n = 0, t = 0, items = 0;                       // stages, tiles and items so far, the other warp's among them
             bool ok = true, fresh = true;
             constexpr uint32_t kIdesc = ((uint32_t)(kPairCols >> 3) << 17) | (1u << 23) | ((uint32_t)(kPairLanes >> 4) << 24);
-            const uint32_t base = smem_u32(tiles), power = smem_u32(s_power), sf_power = tmem + kSf + kStages * S::kSlot;
+            const uint32_t base = smem_u32(tiles), power = smem_u32(s_power), sf_power = tmem + kSf + kStages * S::kSlot + 4 * own;
             for (int64_t at = first; at < last && ok;) {
                 const PairSpan sp = pair_span<S::kNorms>(job, at, last);
                 at = sp.next;
