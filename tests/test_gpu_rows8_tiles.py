@@ -55,3 +55,35 @@ def test_every_digit_of_a_centres_norm(dim):
         got.append(coverage(zeros, c.take(pick)))
     got = torch.stack(got)
     assert torch.equal(got, norms[:, None].expand(k, 3))
+
+
+# ---- products of many rows with many: pairs of SMs --------------------------------------------------------------
+
+@pytest.mark.parametrize("n,k", [(4096, 8192), (4001, 8191)])          # bulk stores, and the readers' own
+@pytest.mark.parametrize("dim", [16, 40, 128, 256, 384, 1024, 2050])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_products_of_many_tiles_are_exact(n, k, dim, dtype):
+    (a, x), (b, y) = stored(n, dim, n + dim, powers=True), stored(k, dim, k, powers=True)
+    assert torch.equal(row_products(a, b, dtype=dtype), ex.products(x, y).float().to(dtype))
+    a.check_status()
+
+
+# ---- at most 64 columns: single SMs ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("k", [1, 9, 16, 20, 32, 33, 64])
+@pytest.mark.parametrize("n,dim", [(200_000, 16), (200_003, 30), (200_000, 50), (200_003, 128), (200_000, 300), (50_001, 1100)])
+def test_few_columns_of_many_tiles_are_exact(n, k, dim):
+    (a, x), (b, y) = stored(n, dim, n + dim), stored(k, dim, k)
+    want = ex.distances(x, y)
+    assert torch.equal(coverage(a, b).double(), want)
+    h = torch.where(torch.arange(n, device="cuda") % 3 == 0, want / 2, float("inf")).float()
+    h[5::7] = -1.0
+    prior = h.double()
+    coverage(a, b, h=h)
+    assert torch.equal(h.double(), torch.minimum(prior, want))
+    want = ex.products(x, y).float()
+    for dtype in (torch.float32, torch.bfloat16):
+        assert torch.equal(row_products(a, b, dtype=dtype), want.to(dtype))       # rows of the result follow the columns
+        assert torch.equal(row_products(b, a, dtype=dtype), want.T.to(dtype))     # and the lanes
+    a.check_status()
+    b.check_status()
