@@ -360,7 +360,7 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                 const float d = __fadd_rn(row_norm, fminf(fminf(best[0], best[1]), fminf(best[2], best[3])));
                 const float up = d == d ? fmaxf(d, 0.0f) : __uint_as_float(0x7f800000u);
                 float* h = reinterpret_cast<float*>(job.out) + row;
-                *h = job.keep ? fminf(*h, up) : up;
+                if (!job.keep || up < *h) *h = up;      // (a NaN there stays)
             }
         }
         if (WHAT == R8_PRODUCTS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

@@ -359,7 +359,16 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             at = sp.next;
             const int64_t row = sp.lt * kPairLanes + rank * kR8Lanes + quad * 32 + lane;
             float best[4] = {low, low, low, low};
-            const float row_norm = WHAT == R8_COVERAGE && row < job.n_lane ? __ldg(job.lane_norms + row) : 0.0f;     // (ahead of the tiles)
+            float row_norm = 0.0f;                                  // (ahead of the tiles)
+            if (WHAT == R8_COVERAGE && row < job.n_lane) {
+                row_norm = __ldg(job.lane_norms + row);
+                // a NaN in h stays: its row's distances become NaN too.  No pair ever lowers a NaN, so whether there is one does
+                // not depend on when this looks
+                if (job.keep) {
+                    const float had = __ldcg(reinterpret_cast<const float*>(job.out) + row);
+                    row_norm = had == had ? row_norm : had;
+                }
+            }
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct, ++t) {
                 const uint32_t buf = t & 1u;
                 ok = r8_wait_warp(&s_acc_full[buf], (t >> 1) & 1u, s_abort);

@@ -446,9 +446,10 @@ CS_API int cs_rows8_products(const cs_rows8* a, const cs_rows8* b, void* out, in
                              cs_stream stream);
 
 /* h[i] = min over the centres j of max(0, norms_a[i] + norms_c[j] - 2 dot(i, j)), i in [0, a->count); with
- * keep != 0 also over what h[i] holds (rows that carry -1 keep it).  A distance that is NaN never lowers
- * h; without centres h is +inf (keep == 0).  `work` is cs_rows8_coverage_bytes(centres->count) bytes of scratch,
- * 16-byte aligned (0 bytes: may be NULL).  At most 2^30 - 1024 centres (CS_E_RANGE). */
+ * keep != 0 also over what h[i] holds (rows that carry -1 keep it, and so do rows that carry a NaN).  A
+ * distance that is NaN never lowers h; without centres h is +inf (keep == 0).  `work` is
+ * cs_rows8_coverage_bytes(centres->count) bytes of scratch, 16-byte aligned (0 bytes: may be NULL).  At
+ * most 2^30 - 1024 centres (CS_E_RANGE). */
 CS_API int64_t cs_rows8_coverage_bytes(int64_t n_centres);
 CS_API int cs_rows8_coverage(const cs_rows8* a, const cs_rows8* centres, float* h, int32_t keep, void* work,
                              cs_stream stream);
