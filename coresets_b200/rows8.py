@@ -22,6 +22,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _native
 from ._native import CsRows8
@@ -213,6 +214,7 @@ def quantise_rows(X: Tensor, *, store: Optional[RowStore] = None, start: Optiona
     if (dim > 1 and X.stride(1) != 1) or (n > 1 and X.stride(0) < dim):
         X = X.contiguous()
     _call(store.device, "cs_rows8_write", store._ref, X.data_ptr(), code, n, X.stride(0) if n > 1 else dim, start)
+    increment_version((store._codes, store._scales, store._norms))        # (autograd cannot know of writes through addresses)
     if start + n > store._c.count:
         store._c.count = start + n
     return store
@@ -241,10 +243,13 @@ def read_rows(store: RowStore, rows=None, *, dtype: torch.dtype = torch.float32,
     if rows is not None:
         rows = _row_numbers(store, rows)
     m = store.count if rows is None else rows.shape[0]
+    given = out is not None
     out = _result(out, (m, store.dim), dtype, store._norms)
     if m:
         _call(store.device, "cs_rows8_read", store._ref, None if rows is None else rows.data_ptr(), m, out.data_ptr(), code,
               out.stride(0) if m > 1 else store.dim)
+        if given:
+            increment_version(out)
     return out
 
 
@@ -269,9 +274,12 @@ def row_products(a: RowStore, b: RowStore, *, dtype: torch.dtype = torch.float32
     _check_pair(a, b, ("a", "b"))
     code = _dtype_code(dtype, "dtype")
     n, k = a.count, b.count
+    given = out is not None
     out = _result(out, (n, k), dtype, a._norms)
     if n and k:
         _call(a.device, "cs_rows8_products", a._ref, b._ref, out.data_ptr(), code, out.stride(0) if n > 1 else k)
+        if given:
+            increment_version(out)
     return out
 
 
@@ -302,6 +310,8 @@ def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
         size = _native.get_native().lib.cs_rows8_coverage_bytes(centres.count)
         work = store._norms.new_empty(size >> 2) if size else None
         _call(store.device, "cs_rows8_coverage", store._ref, centres._ref, h.data_ptr(), int(keep), work.data_ptr() if size else None)
+        if keep:
+            increment_version(h)
     return h
 
 

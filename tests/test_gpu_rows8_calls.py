@@ -32,3 +32,26 @@ def test_a_nan_in_h_stays(k):
     z = a.take(torch.full((1000,), -1, device="cuda"))
     coverage(z, c, h=h)
     assert torch.equal(h.isnan(), nan) and torch.equal(h[~nan].double(), want[~nan])
+
+
+def test_writes_move_the_version_counter():
+    """A graph that saved a tensor which a call then wrote to must not be differentiated with the new values."""
+    (a, x), (c, _) = stored(300, 40, 1), stored(20, 40, 2)
+
+    def saved(t):
+        w = torch.ones_like(t, requires_grad=True)
+        return (w * t).sum()
+    h, wide = torch.zeros(300, device="cuda"), torch.zeros(300, 60, device="cuda")
+    for t, call in ((h, lambda: coverage(a, c, h=h)), (wide, lambda: read_rows(a, out=wide[:, 3:43])), (wide, lambda: row_products(a, c, out=wide[:, :20])),
+                    (a.norms, lambda: quantise_rows(x, store=a, start=0))):
+        y, before = saved(t), t._version
+        call()
+        assert t._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    codes, scales = a.codes._version, a.scales._version
+    quantise_rows(x[:1], store=a, start=0)
+    assert a.codes._version > codes and a.scales._version > scales
+    with torch.inference_mode():                          # (such tensors have no counter)
+        t = torch.zeros(300, device="cuda")
+    assert torch.equal(coverage(a, c, h=t), torch.zeros(300, device="cuda"))
