@@ -178,9 +178,9 @@ int launch_rows8_pair(const cs_rows8* lanes, const cs_rows8* cols, R8Job& job, v
         const int64_t rows = r8_norm_rows(job.n_col);
         unsigned char* digits = static_cast<unsigned char*>(work);
         unsigned char* scales = digits + rows * 16;
-        const int64_t n_h = job.keep ? 0 : job.n_lane, most = rows > n_h ? rows : n_h;
-        rows8_norm_digits_kernel<<<r8_grid((most + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(job.col_norms, job.n_col, rows, digits, scales,
-                                                                                                 static_cast<float*>(job.out), n_h);
+        const int64_t most = rows > job.n_lane ? rows : job.n_lane;
+        rows8_norm_digits_kernel<<<r8_grid((most + kThreads - 1) / kThreads, d), kThreads, 0, st>>>(
+            job.col_norms, job.n_col, rows, digits, scales, static_cast<float*>(job.out), job.n_lane, job.keep);
         rc = check_launch();
         if (!rc) rc = r8_map(&maps.norm, digits, 16, rows, 16, kPairCols / 2);
         if (!rc) rc = r8_scale_map(&maps.norm_sf, scales, 1, rows, 2);

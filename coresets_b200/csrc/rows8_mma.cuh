@@ -294,7 +294,11 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
             if (t % S::kSets != (uint32_t)set) continue;
             const int64_t row = item * kR8Lanes + quad * 32 + lane;
             const uint32_t buf = t % S::kAcc;
-            const float row_norm = WHAT == R8_COVERAGE && row < job.n_lane ? __ldg(job.lane_norms + row) : 0.0f;      // (ahead of the wait)
+            float row_norm = 0.0f, had = __uint_as_float(0x7f800000u);      // (ahead of the wait)
+            if (WHAT == R8_COVERAGE && row < job.n_lane) {
+                row_norm = __ldg(job.lane_norms + row);
+                if (job.keep) had = reinterpret_cast<const float*>(job.out)[row];
+            }
             ok = r8_wait_warp(&s_acc_full[buf], (t / S::kAcc) & 1u, s_abort);
             if (!ok) break;
             tc_fence_after();
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                 const float d = __fadd_rn(row_norm, fminf(fminf(best[0], best[1]), fminf(best[2], best[3])));
                 const float up = d == d ? fmaxf(d, 0.0f) : __uint_as_float(0x7f800000u);
                 float* h = reinterpret_cast<float*>(job.out) + row;
-                if (!job.keep || up < *h) *h = up;      // (a NaN there stays)
+                *h = up < had ? up : had;               // (a NaN there stays)
             }
         }
         if (WHAT == R8_PRODUCTS && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");

@@ -291,7 +291,7 @@ def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
     norms, not of itself.
 
     With ``h`` the minimum is taken with what ``h`` holds, in place: a selection can be passed part by part,
-    and rows that carry -1 (selected) keep it, as do rows that carry a NaN.  A distance is never negative, one that is NaN
+    and rows that carry -1 (selected) keep it; rows that carry a NaN stay NaN.  A distance is never negative, one that is NaN
     never lowers ``h``, and without centres a new ``h`` is +inf."""
     _check_store(store, "store")
     if not isinstance(centres, RowStore):

@@ -446,7 +446,7 @@ CS_API int cs_rows8_products(const cs_rows8* a, const cs_rows8* b, void* out, in
                              cs_stream stream);
 
 /* h[i] = min over the centres j of max(0, norms_a[i] + norms_c[j] - 2 dot(i, j)), i in [0, a->count); with
- * keep != 0 also over what h[i] holds (rows that carry -1 keep it, and so do rows that carry a NaN).  A
+ * keep != 0 also over what h[i] holds (rows that carry -1 keep it, rows that carry a NaN stay NaN).  A
  * distance that is NaN never lowers h; without centres h is +inf (keep == 0).  `work` is
  * cs_rows8_coverage_bytes(centres->count) bytes of scratch, 16-byte aligned (0 bytes: may be NULL).  At
  * most 2^30 - 1024 centres (CS_E_RANGE). */
