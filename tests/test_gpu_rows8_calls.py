@@ -55,3 +55,20 @@ def test_writes_move_the_version_counter():
     with torch.inference_mode():                          # (such tensors have no counter)
         t = torch.zeros(300, device="cuda")
     assert torch.equal(coverage(a, c, h=t), torch.zeros(300, device="cuda"))
+
+
+def test_tangents_are_refused():
+    (a, x), (c, _) = stored(30, 40, 1), stored(5, 40, 2)
+    h, out = torch.zeros(30, device="cuda"), torch.zeros(30, 40, device="cuda")
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="gradient"):
+            quantise_rows(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(ValueError, match="gradient"):
+            coverage(a, c, h=forward_ad.make_dual(h, torch.ones_like(h)))
+        with pytest.raises(ValueError, match="gradient"):
+            read_rows(a, out=forward_ad.make_dual(out, torch.ones_like(out)))
+        with pytest.raises(ValueError, match="gradient"):
+            RowStore.from_tensors(a.codes, a.scales, forward_ad.make_dual(a.norms, torch.ones_like(a.norms)), 40)
+        assert torch.equal(read_rows(quantise_rows(x)), x)
+    with pytest.raises(ValueError, match="gradient"):
+        RowStore.from_tensors(a.codes, a.scales, a.norms.clone().requires_grad_(), 40)
