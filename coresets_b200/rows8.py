@@ -49,6 +49,8 @@ def _check_written(t: Tensor, name: str) -> None:
     """A tensor that a call writes to through its address."""
     if t.requires_grad or _has_tangent(t):
         raise ValueError(f"{name} must not require a gradient or carry a tangent (forward mode)")
+    if t.is_neg():
+        raise ValueError(f"{name} must not be a negated view (Tensor.is_neg)")
 
 
 # the current stream's handle without building a Stream object (1.3 us a call)
@@ -228,6 +230,7 @@ def quantise_rows(X: Tensor, *, store: Optional[RowStore] = None, start: Optiona
         return store
     if (dim > 1 and X.stride(1) != 1) or (n > 1 and X.stride(0) < dim):
         X = X.contiguous()
+    X = X.resolve_neg()                     # (a view such as z.conj().imag stands for the negative of its memory)
     _call(store.device, "cs_rows8_write", store._ref, X.data_ptr(), code, n, X.stride(0) if n > 1 else dim, start)
     increment_version((store._codes, store._scales, store._norms))        # (autograd cannot know of writes through addresses)
     if start + n > store._c.count:

@@ -72,3 +72,15 @@ def test_tangents_are_refused():
         assert torch.equal(read_rows(quantise_rows(x)), x)
     with pytest.raises(ValueError, match="gradient"):
         RowStore.from_tensors(a.codes, a.scales, a.norms.clone().requires_grad_(), 40)
+
+
+def test_negated_views():
+    """A view that stands for the negative of its memory is read as that, and not written to."""
+    z = torch.complex(torch.arange(40.0), torch.arange(1.0, 41.0)).cuda()[:, None]
+    x = z.conj().imag
+    assert x.is_neg()
+    assert torch.equal(read_rows(quantise_rows(x)), read_rows(quantise_rows(x.clone())))
+    with pytest.raises(ValueError, match="negated"):
+        read_rows(quantise_rows(x.clone()), out=z.conj().imag)
+    with pytest.raises(ValueError, match="negated"):
+        coverage(quantise_rows(x[:1].clone()), [0], h=torch._neg_view(torch.zeros(1, device="cuda")))
