@@ -165,10 +165,14 @@ class RowStore:
         return out
 
     def check_status(self) -> None:
-        """Synchronise and raise if a bounded wait inside a ``row_products`` or ``coverage`` with this store as its first
-        argument ran out."""
+        """Wait for everything on the device (the calls may have been made on any stream) and raise if a bounded wait
+        inside a ``row_products`` or ``coverage`` with this store as its first argument has run out since the last time this
+        was asked.  Those calls cannot tell by themselves: they do not wait for what they enqueue."""
+        torch.cuda.synchronize(self.device)
         status = int(self._status.item())
         if status:
+            self._status.zero_()
+            torch.cuda.synchronize(self.device)         # (cleared before another stream may set it)
             raise RuntimeError(f"a bounded wait of a product over {self!r} ran out (status {status}); its result is not valid")
 
 
@@ -281,7 +285,7 @@ def _check_pair(a: RowStore, b: RowStore, names) -> None:
 
 def row_products(a: RowStore, b: RowStore, *, dtype: torch.dtype = torch.float32, out: Optional[Tensor] = None) -> Tensor:
     """``[len(a), len(b)]``: the dot product of every row of ``a`` with every row of ``b``, summed in the tensor cores'
-    float32 accumulators and rounded once to ``dtype``.
+    float32 accumulators and rounded once to ``dtype``.  (Its waits inside the kernel are bounded: ``a.check_status()``.)
 
     The accumulators cut off (toward zero) instead of rounding, once per 32 elements: each time by less than 2^-23 of the
     sum so far, and terms under 2^-17 of it by less than 2^-25 of it.  So the error of a sum whose terms have one sign has one
@@ -305,7 +309,7 @@ def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
     numbers of rows of this one); its maximum is the squared Hausdorff radius of the selection.
 
     The products behind it are summed as ``row_products`` says, the norms in float32: a distance is off by a share of the
-    norms, not of itself.
+    norms, not of itself.  (Bounded waits: ``store.check_status()``.)
 
     With ``h`` the minimum is taken with what ``h`` holds, in place: a selection can be passed part by part,
     and rows that carry -1 (selected) keep it; rows that carry a NaN stay NaN.  A distance is never negative, one that is NaN

@@ -84,3 +84,21 @@ def test_negated_views():
         read_rows(quantise_rows(x.clone()), out=z.conj().imag)
     with pytest.raises(ValueError, match="negated"):
         coverage(quantise_rows(x[:1].clone()), [0], h=torch._neg_view(torch.zeros(1, device="cuda")))
+
+
+@pytest.mark.parametrize("n,k", [(300, 5), (300, 200)])
+def test_the_status_is_reported_once(n, k):
+    """Also of a call on another stream than the one that asks."""
+    (a, x), (c, y) = stored(n, 300, 1), stored(k, 300, 2)
+    side = torch.cuda.Stream()
+    for call in (row_products, coverage):
+        torch.cuda.synchronize()
+        a._c.flags = c._c.flags = _native.ROWS8_TEST_STALL
+        with torch.cuda.stream(side):
+            call(a, c)
+        a._c.flags = c._c.flags = 0
+        with pytest.raises(RuntimeError, match="ran out"):
+            a.check_status()
+        a.check_status()
+        assert torch.equal(coverage(a, c).double(), ex.distances(x, y))
+        a.check_status()
