@@ -12,8 +12,13 @@ float32.  The rounding to e4m3 is off by at most 2^-4 of an element, or 2^-10 of
 the rows as stored, with float32 sums, those of products in the tensor cores' accumulators (see ``row_products``).
 
 Every call is enqueued on the current stream of the store's device, allocates nothing but its result (and a
-contiguous copy of an input whose columns are strided, and 20 bytes of scratch per centre), synchronises with nothing and can be captured into
-a CUDA graph.
+contiguous copy of an input whose columns are strided, and 20 bytes of scratch per centre of more than 64), synchronises
+with nothing and can be captured into a CUDA graph.  Beyond that:
+
+* row numbers that the host holds are checked and copied to the device, for which the host waits: they are refused while the
+  stream is capturing;
+* ``coverage`` by row numbers first takes these rows into a store of their own;
+* ``fps_cuda`` reads the rows back into a matrix (``store_matrix``) and returns when it has selected; ``check_status`` waits.
 """
 from __future__ import annotations
 
@@ -187,6 +192,10 @@ def _row_numbers(store: RowStore, rows) -> Tensor:
     if not rows.is_cuda:
         if rows.numel() and not (0 <= int(rows.min()) and int(rows.max()) < store.count):
             raise IndexError(f"rows must be in [0, {store.count}), got {int(rows.min())} .. {int(rows.max())}")
+        if rows.numel():
+            with torch.cuda.device(store.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise ValueError("row numbers on the host cannot be captured into a graph: pass them on the device")
     elif rows.device != store.device:
         raise ValueError(f"rows are on {rows.device}, the store on {store.device}")
     return rows.to(device=store.device, dtype=torch.int64).contiguous()

@@ -102,3 +102,18 @@ def test_the_status_is_reported_once(n, k):
         a.check_status()
         assert torch.equal(coverage(a, c).double(), ex.distances(x, y))
         a.check_status()
+
+
+def test_row_numbers_of_the_host_are_refused_while_capturing():
+    (a, x), (c, _) = stored(300, 40, 1), stored(70, 40, 2)
+    pick = torch.tensor([5, 299, 0], device="cuda")
+    coverage(a, pick)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for call in (lambda: read_rows(a, [5, 299, 0]), lambda: a.take(torch.tensor([5])), lambda: coverage(a, [5])):
+            with pytest.raises(ValueError, match="captur"):
+                call()
+        got = read_rows(a, pick)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, x[pick])
