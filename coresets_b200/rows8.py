@@ -190,6 +190,7 @@ def _row_numbers(store: RowStore, rows) -> Tensor:
     if rows.dim() != 1 or rows.dtype.is_floating_point or rows.dtype.is_complex or rows.dtype == torch.bool:
         raise ValueError(f"rows must be a 1-D tensor of whole numbers, got {rows.dtype} of shape {tuple(rows.shape)}")
     if not rows.is_cuda:
+        rows = rows.to(torch.int64)                     # (wide unsigned types have no minimum)
         if rows.numel() and not (0 <= int(rows.min()) and int(rows.max()) < store.count):
             raise IndexError(f"rows must be in [0, {store.count}), got {int(rows.min())} .. {int(rows.max())}")
         if rows.numel():

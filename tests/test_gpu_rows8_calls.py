@@ -117,3 +117,13 @@ def test_row_numbers_of_the_host_are_refused_while_capturing():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, x[pick])
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int16, torch.int32, torch.uint16, torch.uint32, torch.uint64])
+def test_row_numbers_of_every_type(dtype):
+    a, x = stored(250, 40, 1)
+    pick = torch.tensor([5, 249, 0])
+    assert torch.equal(read_rows(a, pick.to(dtype)), x[pick.cuda()])
+    assert torch.equal(read_rows(a, pick.to(dtype).cuda()), x[pick.cuda()])
+    with pytest.raises(IndexError):
+        read_rows(a, torch.tensor([5, 250]).to(dtype))

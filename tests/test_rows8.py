@@ -7,6 +7,7 @@ import torch
 
 import coresets_b200 as coresets
 from coresets_b200 import _native, build
+from coresets_b200.rows8 import _row_numbers
 from tests import rows8_oracle as ref
 
 
@@ -97,3 +98,13 @@ def test_c_abi_refusals(lib):
     assert lib.cs_rows8_read(r(none), None, 0, None, 0, 64, None) == 0
     assert lib.cs_rows8_products(r(none), r(good), None, 0, 50, None) == 0
     assert lib.cs_rows8_coverage(r(none), r(good), None, 0, None, None) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.uint16, torch.uint32, torch.uint64])
+def test_row_numbers_out_of_range_of_every_type(dtype):
+    store = type("Store", (), {"device": torch.device("cuda", 0), "count": 50})()
+    for bad in ([3, 50], [100]):
+        with pytest.raises(IndexError, match=r"\[0, 50\)"):
+            _row_numbers(store, torch.tensor(bad).to(dtype))
+        with pytest.raises(IndexError, match=r"\[0, 50\)"):
+            _row_numbers(store, np.array(bad).astype(str(dtype).split(".")[1]))
