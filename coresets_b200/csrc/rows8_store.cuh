@@ -6,7 +6,8 @@
 //   code = e4m3(x * 2^-e), to nearest, ties to even; NaN and infinities become the NaN code
 // so a scale is a power of two: x * 2^-e is exact, and so is code * 2^e in float32 and bfloat16 (4
 // significant bits; e >= -117 keeps the smallest non-zero value, 2^-126, a normal float32).  The only
-// rounding of a write is the one to e4m3 (relative 2^-4 in the normal range of the block).
+// rounding of a write is the one to e4m3 (relative 2^-4 in the normal range of the block).  Magnitudes of 248 * 2^120 and
+// more round to 256 * 2^120, past float32: such a code reads as infinity.
 #ifndef CORESETS_B200_ROWS8_STORE_CUH
 #define CORESETS_B200_ROWS8_STORE_CUH
 

@@ -215,7 +215,8 @@ def quantise_rows(X: Tensor, *, store: Optional[RowStore] = None, start: Optiona
     (default: behind the rows it holds), over what stands there; the store has to have room for them and no
     row before ``start`` may be unwritten.  Per block of 128 elements the scale is 2^e with the least e >= -117
     for which every finite element fits e4m3 (448 at most); elements are rounded to nearest, ties to even.
-    NaN and infinities are stored as NaN.  No gradient flows through."""
+    NaN and infinities are stored as NaN.  Magnitudes from 248 * 2^120 (3.3e38) to the largest float32 round to 2^128, which
+    the store holds but float32 and bfloat16 do not: they are read as infinity.  No gradient flows through."""
     if X.dim() != 2:
         raise ValueError(f"X must be 2-D (N, D), got shape {tuple(X.shape)}")
     if not X.is_cuda:
@@ -265,7 +266,8 @@ def _result(out: Optional[Tensor], shape, dtype, like: Tensor) -> Tensor:
 
 
 def read_rows(store: RowStore, rows=None, *, dtype: torch.dtype = torch.float32, out: Optional[Tensor] = None) -> Tensor:
-    """Rows of the store as ``dtype`` (exact in float32 and bfloat16, rounded once in float16).
+    """Rows of the store as ``dtype`` (exact in float32 and bfloat16 but for 2^128, which is infinity there; rounded once in
+    float16).
 
     ``rows``: whole numbers in any order, repeats allowed; default all rows.  Numbers that the host holds are
     checked (``IndexError``); numbers on the device are not, and one outside ``[0, count)`` gives a row of NaN."""

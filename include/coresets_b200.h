@@ -424,12 +424,13 @@ typedef struct cs_rows8 {
 /* Quantise n rows of X (dtype CS_DTYPE_*, row stride ld elements) into rows start .. start + n of the
  * store (start + n <= capacity; `count` is not looked at).  e = the least integer with amax <= 448 * 2^e
  * over the block's finite elements, at least -117; code = e4m3(x * 2^-e) to nearest even; NaN and
- * infinities become the NaN code.  Other rows are left as they were. */
+ * infinities become the NaN code.  (Magnitudes of 248 * 2^120 and more are stored as 2^128 and read as
+ * infinity.)  Other rows are left as they were. */
 CS_API int cs_rows8_write(const cs_rows8* r, const void* X, int32_t dtype, int64_t n, int64_t ld, int64_t start,
                           cs_stream stream);
 
 /* out[i] = row rows[i] of the store (rows NULL: row i), m rows of row stride ld elements, rounded once to
- * the output type.  A row number outside [0, count) gives a row of NaN. */
+ * the output type (nothing to round in float32 and bfloat16).  A row number outside [0, count) gives a row of NaN. */
 CS_API int cs_rows8_read(const cs_rows8* r, const int64_t* rows, int64_t m, void* out, int32_t dtype, int64_t ld,
                          cs_stream stream);
 

@@ -127,3 +127,18 @@ def test_row_numbers_of_every_type(dtype):
     assert torch.equal(read_rows(a, pick.to(dtype).cuda()), x[pick.cuda()])
     with pytest.raises(IndexError):
         read_rows(a, torch.tensor([5, 250]).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_numbers_are_stored_as_two_to_the_128(dtype):
+    """248 * 2^120 and more round to 256 * 2^120, which float32 and bfloat16 do not have."""
+    top = 2.0 ** 120
+    x = torch.zeros(4, 200, dtype=torch.float64)
+    x[0, 0], x[1, 0], x[2, 150], x[3, 7] = 247 * top, -248 * top, torch.finfo(dtype).max, 240 * top
+    x = x.to(dtype)
+    a = quantise_rows(x.cuda())
+    assert torch.isfinite(x).all() and not a.codes.float().isnan().any()
+    for out in (torch.float32, torch.bfloat16):
+        got = read_rows(a, dtype=out).double().cpu()
+        assert got[3, 7] == 240 * top and got[2, 150] == float("inf") and not got.isnan().any()
+        assert got[0, 0] == (240 * top if x[0, 0].double() < 248 * top else float("inf")) and got[1, 0] == float("-inf")
