@@ -142,3 +142,38 @@ def test_the_largest_numbers_are_stored_as_two_to_the_128(dtype):
         got = read_rows(a, dtype=out).double().cpu()
         assert got[3, 7] == 240 * top and got[2, 150] == float("inf") and not got.isnan().any()
         assert got[0, 0] == (240 * top if x[0, 0].double() < 248 * top else float("inf")) and got[1, 0] == float("-inf")
+
+
+def test_graphs_and_calls_at_once():
+    """Two graphs, each with a coverage of its own (scratch of other norms), replayed on two streams at the same time, beside eager calls."""
+    (a, x), (c, y), (e, z) = stored(20000, 200, 1), stored(600, 200, 2), stored(900, 200, 3)
+    e2 = RowStore.from_tensors(e.codes, e.scales, e.norms, 200, count=431)
+    pick = torch.arange(0, 20000, 97, device="cuda")
+    want = [ex.distances(x, y), ex.distances(x, z), ex.distances(x, x[pick]), ex.distances(x, z[:431])]
+    calls = [lambda: coverage(a, c), lambda: coverage(a, e), lambda: coverage(a, pick), lambda: coverage(a, e2)]
+    for call in calls:
+        call()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([calls[i](), calls[i + 2]()])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for out in outs:
+            for t in out:
+                t.fill_(-5.0)
+        torch.cuda.synchronize()
+        eager = []
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+            with torch.cuda.stream(streams[2 + i]):
+                eager.append((calls[i](), calls[i + 2]()))
+        torch.cuda.synchronize()
+        for i in range(2):
+            for got in (outs[i], eager[i]):
+                assert torch.equal(got[0].double(), want[i]) and torch.equal(got[1].double(), want[i + 2])
+    a.check_status()
