@@ -183,7 +183,7 @@ class RowStore:
 
 def _row_numbers(store: RowStore, rows) -> Tensor:
     if not isinstance(rows, Tensor):
-        rows = torch.as_tensor(rows)
+        rows = torch.as_tensor(rows, device="cpu")       # (whatever the default device: these are checked)
         rows = rows.to(torch.int64) if rows.numel() == 0 else rows
     if rows.dtype == torch.int64 and rows.dim() == 1 and rows.device == store.device and rows.is_contiguous():
         return rows

@@ -108,3 +108,9 @@ def test_row_numbers_out_of_range_of_every_type(dtype):
             _row_numbers(store, torch.tensor(bad).to(dtype))
         with pytest.raises(IndexError, match=r"\[0, 50\)"):
             _row_numbers(store, np.array(bad).astype(str(dtype).split(".")[1]))
+
+
+def test_row_numbers_of_a_list_are_the_hosts_under_another_default_device():
+    store = type("Store", (), {"device": torch.device("cuda", 0), "count": 50})()
+    with torch.device("meta"), pytest.raises(IndexError, match="50 .. 50"):
+        _row_numbers(store, [50])
