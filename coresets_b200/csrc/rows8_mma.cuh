@@ -160,11 +160,13 @@ template <int NT, int WHAT, typename T> struct R8Shape {
     static constexpr int kAcc = 256 / (NT < 32 ? 32 : NT);             // accumulators: 8, 8, 4; the way from a tile's last MMA to its
                                                                        // free accumulator is much longer than its few MMAs
     // Sets of four reading warps (a set has the tile's 128 lanes), tile by tile in turn: a reader's way from accumulator to
-    // memory is long, and what a tile takes else is short (461k x 10 x 16 to float16: 39 us with one set, 34 with four; 1M x 64 x 128: coverage 49 -> 33).  kAcc
-    // is a multiple of it, so that the wait for an accumulator's fill comes after the same set's wait for the fill before.
+    // memory is long, and what a tile takes else is short (461k x 10 x 16 to float16: 39 us with one set, 34 with four;
+    // 1M x 64 x 128: coverage 49 -> 33).  kAcc is a multiple of it, so that the wait for an accumulator's fill comes after the
+    // same set's wait for the fill before.
     static constexpr int kSets = kAcc / 2;
     static constexpr int kThreads = 64 + 128 * kSets;
-    static constexpr int kOutWarp = WHAT == R8_PRODUCTS ? (32 * (NT + 1) * (int)sizeof(T) + 127) & ~127 : 0;      // a reader's products on their way out
+    // a reader's products on their way out
+    static constexpr int kOutWarp = WHAT == R8_PRODUCTS ? (32 * (NT + 1) * (int)sizeof(T) + 127) & ~127 : 0;
     static constexpr int kOut = 4 * kSets * kOutWarp;
     static constexpr int kFit = (226 * 1024 - kOut - 1024 - 2048) / kStage;
     static constexpr int kStages = kFit < 8 ? kFit : 8;
@@ -236,7 +238,8 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
             }
         }
         // the last releases of the stages have arrived before the block leaves
-        for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n && ok; ++k) ok = r8_wait_warp(&s_empty[k % S::kStages], (k / S::kStages) & 1u, s_abort);
+        for (uint32_t k = n > S::kStages ? n - S::kStages : 0; k < n && ok; ++k)
+            ok = r8_wait_warp(&s_empty[k % S::kStages], (k / S::kStages) & 1u, s_abort);
         // no copy may be in flight when the block leaves: the last fills of every stage (already
         // complete unless a consumer gave up)
         if (!ok)
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__((R8Shape<NT, WHAT, T>::kThreads), 1) rows8_mma
                 T* mine = reinterpret_cast<T*>(tiles + S::kStages * S::kStage + reader * S::kOutWarp);
                 if (job.bulk_out) {
                     // NT columns x 32 lanes through shared memory, one bulk store for the warp
-                                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < NT; ++j) r8_narrow(mine[j * 32 + lane], __uint_as_float(v[j]));

@@ -35,7 +35,8 @@ template <int WHAT, typename T, bool KEEP> struct PairShape {
     static constexpr int kStages = KEEP ? 5 : (!kNorms && sizeof(T) == 4 ? 4 : 6);
     static constexpr int kTile = (KEEP ? 0 : kPairA) + kPairB;                 // codes of a stage
     static constexpr int kKept = KEEP ? kPairKept * kPairA : 0;                // lane operand of whole segments
-    static constexpr int kFirst = (kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0) + 127) & ~127;    // what else a stage may bring in (digits end with 16 zero bytes)
+    // what else a stage may bring in (digits end with 16 zero bytes)
+    static constexpr int kFirst = (kPairSf + (kNorms ? kPairNormSf + kPairNormB + 16 : 0) + 127) & ~127;
     static constexpr int kSmem = kKept + kStages * (kTile + kFirst) + kOut + 1024;
     // TMEM columns of scales, one slot per 4 blocks of a row.  A slot comes round after kStages groups of at least one stage:
     // the last stage of the group that had it was filled again, so its MMAs are done, before the group that gets it was.
@@ -184,15 +185,24 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
     if (threadIdx.x == 0) {
         s_abort_word = 0;
         for (int i = 0; i < kStages; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&s_acc_full[i], 1); mbar_init(&s_acc_empty[i], 2 * kPairReaders); mbar_init(&s_kept_full[i], 1); mbar_init(&s_kept_empty[i], two ? 2 : 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_acc_full[i], 1);
+            mbar_init(&s_acc_empty[i], 2 * kPairReaders);
+            mbar_init(&s_kept_full[i], 1);
+            mbar_init(&s_kept_empty[i], two ? 2 : 1);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (S::kNorms) {
         // 128 equal rows of 32 codes without a swizzle: 16 bytes of a row, 8 rows a group; the second 16 are 0
-        for (int i = threadIdx.x; i < (4096 + 512) / 4; i += blockDim.x)
-            reinterpret_cast<unsigned*>(s_power)[i] = i >= 1024 ? 0x70707070u : (i < 512 && (i & 3) == 0 ? 0x50301001u : (i < 512 && (i & 3) == 1 ? 0x7070u : 0u));
-        if (threadIdx.x < kStages * 4)
-            *reinterpret_cast<unsigned*>(tiles + kStages * S::kTile + (threadIdx.x >> 2) * S::kFirst + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
+        for (int i = threadIdx.x; i < (4096 + 512) / 4; i += blockDim.x) {
+            const unsigned codes = i < 512 && (i & 3) == 0 ? 0x50301001u : (i < 512 && (i & 3) == 1 ? 0x7070u : 0u);
+            reinterpret_cast<unsigned*>(s_power)[i] = i >= 1024 ? 0x70707070u : codes;
+        }
+        if (threadIdx.x < kStages * 4) {
+            unsigned char* first = tiles + kStages * S::kTile + (threadIdx.x >> 2) * S::kFirst;
+            *reinterpret_cast<unsigned*>(first + kPairSf + kPairNormSf + kPairNormB + 4 * (threadIdx.x & 3)) = 0u;
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     const int width = NARROW ? job.width : kR8Block;
@@ -240,10 +250,15 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
             for (int ct = sp.c0; ct < sp.c1 && ok; ++ct)
                 for (int kb = 0; kb < kblocks; ++kb, ++n) {
                     if (n >= kStages && !r8_wait_warp(&s_empty[st], phase ^ 1u, s_abort)) { ok = false; break; }
-                    const uint32_t a = smem_u32(tiles + st * S::kTile), sf = smem_u32(tiles + kStages * S::kTile + st * S::kFirst), bar = leader_addr(&s_full[st]);
+                    const uint32_t a = smem_u32(tiles + st * S::kTile), sf = smem_u32(tiles + kStages * S::kTile + st * S::kFirst);
+                    const uint32_t bar = leader_addr(&s_full[st]);
                     const bool scales = (kb & 3) == 0;
                     if (elect_one()) {
-                        if (rank == 0) mbar_expect_tx(&s_full[st], 2 * (((KEEP ? 0 : kR8Lanes) + kPairCols / 2) * width + (scales ? kPairSf : 0) + (S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0)));
+                        if (rank == 0) {
+                            const int codes = ((KEEP ? 0 : kR8Lanes) + kPairCols / 2) * width;
+                            const int norms = S::kNorms && kb == 0 ? kPairNormB + kPairNormSf : 0;
+                            mbar_expect_tx(&s_full[st], 2 * (codes + (scales ? kPairSf : 0) + norms));
+                        }
                         const int col = ct * kPairCols + (int)rank * (kPairCols / 2);
                         if (NARROW && width == 16) {
                             if (!KEEP) pair_line(a, &maps.lane, 2 * row, bar);
@@ -305,7 +320,8 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                         tc_fence_after();
                         if (kb > 0 && (kb & 3) == 0 && ++slot == kStages) slot = 0;
                         if (elect_one()) {
-                            const uint32_t b = base + (st + 1) * S::kTile - kPairB, a = KEEP ? kept_at + kb * kPairA : b - kPairA, sf = base + kStages * S::kTile + st * S::kFirst, norm = sf + kPairSf;
+                            const uint32_t b = base + (st + 1) * S::kTile - kPairB, a = KEEP ? kept_at + kb * kPairA : b - kPairA;
+                            const uint32_t sf = base + kStages * S::kTile + st * S::kFirst, norm = sf + kPairSf;
                             const uint32_t sfa = tmem + kSf + slot * S::kSlot, sfb = sfa + 4;
                             // (the lane operand's powers for the norms: by each warp before its own MMAs)
                             if (S::kNorms && fresh) pair_copy_scales(sf_power, umma_desc(power + 4096, 128, 0));
@@ -330,14 +346,17 @@ rows8_pair_kernel(const __grid_constant__ PairMaps maps, const R8Job job) {
                                 const uint64_t da = umma_desc(a, 1024, 2), db = umma_desc(b, 1024, 2);
                                 if (left > 96) {
 #pragma unroll
-                                    for (int k = 0; k < 4; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || kb > 0 || k > 0);
+                                    for (int k = 0; k < 4; ++k)
+                                        pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || kb > 0 || k > 0);
                                 } else {
                                     const int steps = (left + 31) >> 5;
-                                    for (int k = 0; k < steps; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || kb > 0 || k > 0);
+                                    for (int k = 0; k < steps; ++k)
+                                        pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || kb > 0 || k > 0);
                                 }
                             } else {
                                 const uint64_t da = tile_desc(a, width, kR8Lanes * 64), db = tile_desc(b, width, kPairCols / 2 * 64);
-                                for (int k = 0; k < (left + 31) >> 5; ++k) pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || k > 0);
+                                for (int k = 0; k < (left + 31) >> 5; ++k)
+                                    pair_mma(acc, da + 2 * k, db + 2 * k, id, sfa, sfb + sub, S::kNorms || k > 0);
                             }
                             pair_commit(&s_empty[st]);
                             if (kb == kblocks - 1) pair_commit(&s_acc_full[buf]);

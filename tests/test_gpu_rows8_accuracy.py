@@ -34,8 +34,8 @@ def test_products_within_the_steps_error(n, k, dim, kind):
 
 
 @pytest.mark.parametrize("n,k,dim", [
-    (33, 2000, 128), (1000, 33, 100), (1000, 64, 256), (700, 300, 16), (500, 200, 48), (500, 65, 129), (300, 400, 513), (257, 300, 1024), (60, 50, 1100),
-    (60, 70, 1100), (3000, 512, 64), (20, 70, 20011), (70, 80, 4096),
+    (33, 2000, 128), (1000, 33, 100), (1000, 64, 256), (700, 300, 16), (500, 200, 48), (500, 65, 129), (300, 400, 513),
+    (257, 300, 1024), (60, 50, 1100), (60, 70, 1100), (3000, 512, 64), (20, 70, 20011), (70, 80, 4096),
 ])
 def test_coverage_within_the_steps_error(n, k, dim):
     (a, x), (c, y) = stored(n, dim, dim), stored(k, dim, dim + 1)
@@ -69,7 +69,10 @@ def test_coverage_of_single_elements_is_exact(n, dim, k):
 
     def rows(m):
         x = torch.zeros(m, dim, device="cuda")
-        v = (1 + torch.randint(0, 8, (m, 1), generator=g, device="cuda") / 8) * torch.exp2(torch.randint(-3, 4, (m, 1), generator=g, device="cuda").float())
-        return x.scatter_(1, torch.randint(0, dim, (m, 1), generator=g, device="cuda"), v * (1 - 2 * torch.randint(0, 2, (m, 1), generator=g, device="cuda")))
+
+        def whole(low, high):
+            return torch.randint(low, high, (m, 1), generator=g, device="cuda")
+        v = (1 + whole(0, 8) / 8) * torch.exp2(whole(-3, 4).float())
+        return x.scatter_(1, whole(0, dim), v * (1 - 2 * whole(0, 2)))
     x, y = rows(n), rows(k)
     assert torch.equal(coverage(quantise_rows(x), quantise_rows(y)).double(), ex.distances(x, y))

@@ -42,8 +42,8 @@ def test_writes_move_the_version_counter():
         w = torch.ones_like(t, requires_grad=True)
         return (w * t).sum()
     h, wide = torch.zeros(300, device="cuda"), torch.zeros(300, 60, device="cuda")
-    for t, call in ((h, lambda: coverage(a, c, h=h)), (wide, lambda: read_rows(a, out=wide[:, 3:43])), (wide, lambda: row_products(a, c, out=wide[:, :20])),
-                    (a.norms, lambda: quantise_rows(x, store=a, start=0))):
+    for t, call in ((h, lambda: coverage(a, c, h=h)), (wide, lambda: read_rows(a, out=wide[:, 3:43])),
+                    (wide, lambda: row_products(a, c, out=wide[:, :20])), (a.norms, lambda: quantise_rows(x, store=a, start=0))):
         y, before = saved(t), t._version
         call()
         assert t._version > before

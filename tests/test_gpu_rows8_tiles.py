@@ -20,9 +20,11 @@ def stored(n, dim, seed, powers=False):
 
 @pytest.mark.parametrize("n,k,dim", [
     # about 12 tiles a pair, runs cut inside the rows of a segment: two issuing warps (dim <= 256), one, rows not kept (dim > 1024)
-    (20000, 2000, 16), (20000, 2000, 30), (20000, 2000, 50), (20000, 2000, 128), (20000, 1999, 256), (20000, 2000, 384), (20000, 2000, 513), (20000, 2000, 1100),
+    (20000, 2000, 16), (20000, 2000, 30), (20000, 2000, 50), (20000, 2000, 128), (20000, 1999, 256), (20000, 2000, 384),
+    (20000, 2000, 513), (20000, 2000, 1100),
     # several segments a pair: the kept rows are filled again in both slots (dim <= 512) and in the only one
-    (60001, 300, 16), (60001, 300, 40), (60001, 300, 128), (60001, 300, 200), (60001, 300, 512), (60001, 300, 700), (60001, 300, 1024), (60001, 90, 256),
+    (60001, 300, 16), (60001, 300, 40), (60001, 300, 128), (60001, 300, 200), (60001, 300, 512), (60001, 300, 700), (60001, 300, 1024),
+    (60001, 90, 256),
 ])
 def test_coverage_of_many_tiles_is_exact(n, k, dim):
     (a, x), (c, y) = stored(n, dim, n + dim), stored(k, dim, k)
@@ -38,12 +40,14 @@ def test_coverage_of_many_tiles_is_exact(n, k, dim):
 
 @pytest.mark.parametrize("dim", [16, 48, 128, 300, 1100])
 def test_every_digit_of_a_centres_norm(dim):
-    """Rows of zeros are as far from a centre as its norm says, in all 24 bits.  Each column of two tiles in turn has the only centre that is not NaN."""
+    """Rows of zeros are as far from a centre as its norm says, in all 24 bits.  Each column of two tiles in turn has the only
+    centre that is not NaN."""
     k = 384
     zeros = quantise_rows(torch.zeros(3, dim, device="cuda"))
     c, _ = stored(k, dim, 1)
     g = torch.Generator(device="cuda").manual_seed(dim)
-    norms = (torch.randint(0, 1 << 23, (k,), generator=g, device="cuda", dtype=torch.int32) | torch.randint(127 - 60, 127 + 61, (k,), generator=g, device="cuda", dtype=torch.int32) << 23).view(torch.float32)
+    part = torch.randint(0, 1 << 23, (k,), generator=g, device="cuda", dtype=torch.int32)
+    norms = (part | torch.randint(127 - 60, 127 + 61, (k,), generator=g, device="cuda", dtype=torch.int32) << 23).view(torch.float32)
     for i in range(6):                                                    # one digit alone, and all but one
         norms[2 * i] = float(0x800000 | 15 << 4 * i)
         norms[2 * i + 1] = float((0xFFFFFF & ~(15 << 4 * i)) | 0x800000)
