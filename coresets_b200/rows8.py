@@ -135,6 +135,7 @@ class RowStore:
 
     def _adopt(self, codes, scales, norms, dim, count):
         self._codes, self._scales, self._norms = codes, scales, norms      # (read-only: the library holds their addresses)
+        self._written = (codes, scales, norms)
         self.dim, self.capacity, self.device = dim, int(codes.shape[0]), codes.device
         self._status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = CsRows8(codes.data_ptr(), scales.data_ptr(), norms.data_ptr(), self._status.data_ptr(),
@@ -243,11 +244,13 @@ def quantise_rows(X: Tensor, *, store: Optional[RowStore] = None, start: Optiona
         raise ValueError(f"rows {start} .. {start + n} do not fit the store's capacity {store.capacity}")
     if n == 0:
         return store
-    if (dim > 1 and X.stride(1) != 1) or (n > 1 and X.stride(0) < dim):
-        X = X.contiguous()
-    X = X.resolve_neg()                     # (a view such as z.conj().imag stands for the negative of its memory)
-    _call(store.device, "cs_rows8_write", store._ref, X.data_ptr(), code, n, X.stride(0) if n > 1 else dim, start)
-    increment_version((store._codes, store._scales, store._norms))        # (autograd cannot know of writes through addresses)
+    if dim == 1:
+        X = X.resolve_neg()                 # (z.conj().imag stands for the negative of its memory; wider ones are strided)
+    ld, step = X.stride()
+    if (dim > 1 and step != 1) or (n > 1 and ld < dim):
+        X, ld = X.contiguous(), dim
+    _call(store.device, "cs_rows8_write", store._ref, X.data_ptr(), code, n, ld if n > 1 else dim, start)
+    increment_version(store._written)       # (autograd cannot know of writes through addresses)
     if start + n > store._c.count:
         store._c.count = start + n
     return store

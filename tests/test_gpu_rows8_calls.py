@@ -80,6 +80,9 @@ def test_negated_views():
     x = z.conj().imag
     assert x.is_neg()
     assert torch.equal(read_rows(quantise_rows(x)), read_rows(quantise_rows(x.clone())))
+    z2 = torch.complex(torch.ones(20, 6), torch.arange(120.0).view(20, 6)).cuda()
+    for wide in (z2.conj().imag, z2[:1].conj().imag, z2[:, :1].expand(20, 6).conj().imag):
+        assert wide.is_neg() and torch.equal(read_rows(quantise_rows(wide)), read_rows(quantise_rows(wide.clone())))
     with pytest.raises(ValueError, match="negated"):
         read_rows(quantise_rows(x.clone()), out=z.conj().imag)
     with pytest.raises(ValueError, match="negated"):
