@@ -352,7 +352,8 @@ def coverage(store: RowStore, centres, *, h: Optional[Tensor] = None) -> Tensor:
 
 def store_matrix(store: RowStore) -> Tensor:
     """The store's rows as a matrix that the selection kernels read, holding exactly the stored values: float16 where
-    every exponent lets it (2 bytes an element), float32 otherwise.  Reads two numbers back to the host."""
+    every exponent lets it (2 bytes an element), float32 otherwise, also where a block of zeros, which carries the least
+    exponent, is all that does not.  Reads two numbers back to the host."""
     e = store.exponents
     if e.numel():
         low, high = (int(v) - 127 for v in torch.stack(torch.aminmax(e)).tolist())
